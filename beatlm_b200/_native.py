@@ -407,3 +407,48 @@ SIGNATURES.update({
     "bl_comm_aborted": (ctypes.c_int, [ctypes.c_void_p]),
     "bl_comm_destroy": (ctypes.c_int, [ctypes.c_void_p]),
 })
+
+
+ROPE_MAX_PAIRS = 128
+
+
+class PackArgs(ctypes.Structure):
+    _fields_ = [("images", ctypes.c_uint32), ("capacity", ctypes.c_uint32),
+                ("lead", ctypes.c_uint32), ("normalized", ctypes.c_uint32),
+                ("grids", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+                ("image", ctypes.c_void_p), ("positions", ctypes.c_void_p)]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("axes", ctypes.c_uint32),
+                ("sections", ctypes.c_uint32 * 3), ("pairing", ctypes.c_int32),
+                ("shared_ladder", ctypes.c_uint32), ("inverse", ctypes.c_uint32),
+                ("dtype", ctypes.c_int32), ("theta", ctypes.c_double),
+                ("freqs", ctypes.c_void_p), ("x", ctypes.c_void_p),
+                ("x_row_stride", ctypes.c_uint64), ("positions", ctypes.c_void_p),
+                ("pos_row_stride", ctypes.c_uint64), ("out", ctypes.c_void_p),
+                ("out_row_stride", ctypes.c_uint64)]
+
+
+class MaskedAttentionArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint32), ("tokens", ctypes.c_uint32),
+                ("heads", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("last_rows", ctypes.c_uint32),
+                ("scale", ctypes.c_float), ("cap", ctypes.c_float), ("mask", ctypes.c_int32),
+                ("qk_dtype", ctypes.c_int32), ("v_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("qkv", ctypes.c_void_p),
+                ("qkv_row_stride", ctypes.c_uint64), ("out", ctypes.c_void_p),
+                ("out_row_stride", ctypes.c_uint64), ("offsets", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("prefix", ctypes.c_void_p),
+                ("slopes", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("pos_row_stride", ctypes.c_uint64), ("pos_axes", ctypes.c_uint32),
+                ("key_splits", ctypes.c_uint32)]
+
+
+SIGNATURES.update({
+    "bl_pack": (ctypes.c_int, [ctypes.POINTER(PackArgs), ctypes.c_void_p]),
+    "bl_rope": (ctypes.c_int, [ctypes.POINTER(RopeArgs), ctypes.c_void_p]),
+    "bl_masked_attention": (ctypes.c_int, [ctypes.POINTER(MaskedAttentionArgs),
+                                           ctypes.c_void_p]),
+})

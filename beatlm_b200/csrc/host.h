@@ -7,6 +7,7 @@
 
 #include <cstdarg>
 #include <cstdint>
+#include <exception>
 #include <functional>
 #include <utility>
 
@@ -59,6 +60,9 @@ int prepare_layernorm(const bl_layernorm_args& a, Launch* out);
 int prepare_layernorm_rows(const bl_layernorm_args& a, uint32_t row_begin, uint32_t row_end,
                            Launch* out);
 int prepare_patchify(const bl_patchify_args& a, Launch* out);
+int prepare_pack(const bl_pack_args& a, Launch* out);
+int prepare_rope(const bl_rope_args& a, Launch* out);
+int prepare_masked_attention(const bl_masked_attention_args& a, Launch* out);
 
 // Whether launches carry the programmatic-stream-serialisation attribute
 // (on unless the environment sets BEATLM_B200_PDL=0).
@@ -115,6 +119,19 @@ inline int enqueue(const Launch& l, cudaStream_t s) {
     cudaError_t e = l.run(s);
     if (e != cudaSuccess) return fail(BL_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return BL_OK;
+}
+
+// Runs `f` (a body returning a status) so that no C++ exception leaves a C
+// entry point: what a launch's closure can throw is a failed host allocation.
+template <typename F>
+int guarded(const char* what, F&& f) noexcept {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        return fail(BL_ERR_CAPACITY, "%s: %s", what, e.what());
+    } catch (...) {
+        return fail(BL_ERR_CAPACITY, "%s: host exception", what);
+    }
 }
 
 }  // namespace bl

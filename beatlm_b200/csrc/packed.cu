@@ -1,0 +1,302 @@
+// The row maps of a packed batch (images and clips of different sizes one
+// after the other in one token buffer) and rotary positions with several
+// axes on its packed Q and K rows.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "host.h"
+
+namespace bl {
+namespace packed {
+
+// ------------------------------------------------------------------ row maps
+
+// Rows of image i: lead + t h w, 0 where a side is not positive, saturated
+// above `cap` (any larger count fills the buffer all the same), so no product
+// of three 32-bit sides overflows 64 bits.
+__device__ __forceinline__ long long image_rows(const int* g, int lead, long long cap) {
+    const long long t = g[0], h = g[1], w = g[2];
+    if (t <= 0 || h <= 0 || w <= 0) return 0;
+    const long long hw = min(h * w, cap + 1);
+    return min(hw * t, cap + 1) + lead;
+}
+
+// offsets[i] = rows before image i, clamped to the capacity: one block scans
+// the images in chunks of its size with a running total.
+__global__ void __launch_bounds__(1024) pack_offsets_kernel(const int* grids, int images, int lead,
+                                                            long long cap, int* offsets,
+                                                            Status* status) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ long long warp_sum[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long total = 0;
+    if (threadIdx.x == 0) offsets[0] = 0;
+    for (int base = 0; base < images; base += 1024) {
+        const int i = base + threadIdx.x;
+        long long v = i < images ? image_rows(grids + 3ll * i, lead, cap) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+            if (lane >= o) v += u;
+        }
+        if (lane == 31) warp_sum[warp] = v;
+        __syncthreads();
+        long long before = total, all = total;
+        for (int w = 0; w < 32; ++w) {
+            if (w < warp) before += warp_sum[w];
+            all += warp_sum[w];
+        }
+        if (i < images) offsets[i + 1] = static_cast<int>(min(before + v, cap));
+        total = all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0 && total > cap) record_status(status, ST_BAD_ARGS, 0x9A);
+}
+
+// Image and position of each row: a binary search of the offsets (the last
+// image that starts at or before the row, so images without rows are passed
+// over), then the patch's (t, y, x).
+__global__ void __launch_bounds__(256) pack_rows_kernel(const int* grids, const int* offsets,
+                                                        int images, int lead, int normalized,
+                                                        long long cap, int* image, float* pos) {
+    pdl_trigger();
+    pdl_wait();
+    const long long r = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (r >= cap) return;
+    int lo = 0, hi = images;  // offsets[lo] <= r
+    while (lo < hi) {
+        const int mid = lo + (hi - lo + 1) / 2;
+        if (offsets[mid] <= r) lo = mid; else hi = mid - 1;
+    }
+    const bool real = lo < images;
+    if (image != nullptr) image[r] = real ? lo : -1;
+    if (pos == nullptr) return;
+    float c[3] = {0.0f, 0.0f, 0.0f};
+    const long long p = real ? r - offsets[lo] - lead : -1;
+    if (p >= 0) {
+        const int* g = grids + 3ll * lo;
+        const unsigned u = static_cast<unsigned>(p), h = g[1], w = g[2];
+        const unsigned row = u / w, at[3] = {row / h, row % h, u % w};
+        for (int a = 0; a < 3; ++a) {
+            const float n = static_cast<float>(g[a]);
+            c[a] = normalized ? static_cast<float>(2ll * at[a] + 1 - g[a]) / n
+                              : static_cast<float>(at[a]);
+        }
+    }
+    for (int a = 0; a < 3; ++a) pos[3 * r + a] = c[a];
+}
+
+// ------------------------------------------------------------------ rotary
+
+struct RopeParams {
+    long long rows;
+    int heads, head_dim, pairs;
+    int axes, sections[3];  // pairs of each axis
+    int pairing;            // BL_ROPE_*
+    int inverse;
+    const void* x;
+    long long x_stride;
+    void* out;
+    long long out_stride;
+    const float* pos;
+    long long pos_stride;
+    double turn[BL_ROPE_MAX_PAIRS];  // frequency / pi: angles in half turns
+};
+
+template <typename T> __device__ __forceinline__ float up(T v);
+template <> __device__ __forceinline__ float up(float v) { return v; }
+template <> __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T down(float v);
+template <> __device__ __forceinline__ float down(float v) { return v; }
+template <> __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+
+// One block a row: its angles' cosines and sines once, in shared memory, then
+// every head's pairs. The angle is formed in 64 bits in half turns and reduced
+// to [-1, 1] before the 32-bit sincospif, so positions of 10^6 and more lose
+// nothing that the result could hold.
+template <typename T>
+__global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeParams p) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ float cs[BL_ROPE_MAX_PAIRS], sn[BL_ROPE_MAX_PAIRS];
+    const long long r = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
+    T* y = static_cast<T*>(p.out) + r * p.out_stride;
+    for (int j = threadIdx.x; j < p.pairs; j += 256) {
+        const int a = j < p.sections[0] ? 0 : j < p.sections[0] + p.sections[1] ? 1 : 2;
+        double h = static_cast<double>(p.pos[r * p.pos_stride + a]) * p.turn[j];
+        h -= 2.0 * rint(0.5 * h);
+        float s, c;
+        sincospif(static_cast<float>(h), &s, &c);
+        cs[j] = c, sn[j] = p.inverse ? -s : s;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.heads * p.pairs; i += 256) {
+        const int head = i / p.pairs, j = i - head * p.pairs;
+        int lo, hi;
+        if (p.pairing == BL_ROPE_HALF) {
+            lo = j, hi = j + p.pairs;
+        } else if (p.pairing == BL_ROPE_ADJACENT) {
+            lo = 2 * j, hi = lo + 1;
+        } else {
+            const int first = j < p.sections[0] ? 0
+                              : j < p.sections[0] + p.sections[1] ? p.sections[0]
+                                                                  : p.sections[0] + p.sections[1];
+            const int n = j < p.sections[0] ? p.sections[0]
+                          : j < p.sections[0] + p.sections[1] ? p.sections[1]
+                                                              : p.sections[2];
+            lo = first + j, hi = lo + n;
+        }
+        const long long b = static_cast<long long>(head) * p.head_dim;
+        const float u = up(x[b + lo]), v = up(x[b + hi]);
+        y[b + lo] = down<T>(u * cs[j] - v * sn[j]);
+        y[b + hi] = down<T>(v * cs[j] + u * sn[j]);
+    }
+    const int rest = p.head_dim - 2 * p.pairs;  // elements that do not turn
+    if (rest > 0 && static_cast<const void*>(x) != static_cast<const void*>(y))
+        for (int i = threadIdx.x; i < p.heads * rest; i += 256) {
+            const long long e = static_cast<long long>(i / rest) * p.head_dim + 2 * p.pairs + i % rest;
+            y[e] = x[e];
+        }
+}
+
+}  // namespace packed
+
+int prepare_pack(const bl_pack_args& a, Launch* out) {
+    if (a.images == 0 || a.capacity == 0)
+        return fail(BL_ERR_INVALID, "pack: no images or no rows");
+    if (a.images > 0x7FFFFFFEu || a.capacity > 0x7FFFFFFFu || a.lead > 0x7FFFFFFFu)
+        return fail(BL_ERR_UNSUPPORTED, "pack: %u images, %u rows, %u lead rows exceed 32-bit rows",
+                    a.images, a.capacity, a.lead);
+    if (a.grids == nullptr || a.offsets == nullptr)
+        return fail(BL_ERR_INVALID, "pack: null grids or offsets");
+    for (const void* q : {static_cast<const void*>(a.grids), static_cast<const void*>(a.offsets),
+                          static_cast<const void*>(a.image), static_cast<const void*>(a.positions)})
+        if (reinterpret_cast<uintptr_t>(q) & 3u)
+            return fail(BL_ERR_INVALID, "pack: a buffer is not 4-byte aligned");
+    Status* st = status_ptr();
+    const bl_pack_args b = a;
+    out->op = BL_OP_PACK;
+    out->run = [=](cudaStream_t s) {
+        const int n = static_cast<int>(b.images), lead = static_cast<int>(b.lead);
+        const long long cap = b.capacity;
+        cudaError_t e = launch_k(packed::pack_offsets_kernel, dim3(1), dim3(1024), 0, s, b.grids, n,
+                                 lead, cap, b.offsets, st);
+        if (e != cudaSuccess || (b.image == nullptr && b.positions == nullptr)) return e;
+        return launch_k(packed::pack_rows_kernel, dim3(static_cast<unsigned>((cap + 255) / 256)),
+                        dim3(256), 0, s, b.grids, b.offsets, n, lead, static_cast<int>(b.normalized),
+                        cap, b.image, b.positions);
+    };
+    return BL_OK;
+}
+
+namespace {
+
+// Bytes from the first to one past the last element of rows x width values.
+uint64_t span_bytes(uint64_t rows, uint64_t stride, uint64_t width, uint64_t esz) {
+    return ((rows - 1) * stride + width) * esz;
+}
+
+}  // namespace
+
+int prepare_rope(const bl_rope_args& a, Launch* out) {
+    using packed::RopeParams;
+    if (a.rows == 0 || a.heads == 0 || a.head_dim == 0)
+        return fail(BL_ERR_INVALID, "rope: zero dimension");
+    if (a.axes < 1 || a.axes > 3) return fail(BL_ERR_INVALID, "rope: %u axes (1 to 3)", a.axes);
+    uint64_t pairs = 0;
+    for (uint32_t i = 0; i < a.axes; ++i) {
+        if (a.sections[i] == 0) return fail(BL_ERR_INVALID, "rope: axis %u has no pairs", i);
+        pairs += a.sections[i];
+    }
+    if (2 * pairs > a.head_dim)
+        return fail(BL_ERR_INVALID, "rope: %llu pairs in a head of %u", (unsigned long long)pairs,
+                    a.head_dim);
+    if (pairs > BL_ROPE_MAX_PAIRS)
+        return fail(BL_ERR_UNSUPPORTED, "rope: %llu pairs (at most %d)", (unsigned long long)pairs,
+                    (int)BL_ROPE_MAX_PAIRS);
+    if (a.pairing < BL_ROPE_HALF || a.pairing > BL_ROPE_AXIS_HALF)
+        return fail(BL_ERR_INVALID, "rope: pairing %d", a.pairing);
+    if (a.dtype != BL_F32 && a.dtype != BL_F16 && a.dtype != BL_BF16)
+        return fail(BL_ERR_INVALID, "rope: dtype %d", a.dtype);
+    if (a.freqs == nullptr && !(a.theta > 0.0 && std::isfinite(a.theta)))
+        return fail(BL_ERR_INVALID, "rope: theta must be finite and positive");
+    if (a.x == nullptr || a.out == nullptr || a.positions == nullptr)
+        return fail(BL_ERR_INVALID, "rope: null pointer");
+    const uint64_t esz = dtype_size(a.dtype), width = 1ull * a.heads * a.head_dim;
+    const uint64_t xs = a.x_row_stride ? a.x_row_stride : width;
+    const uint64_t os = a.out_row_stride ? a.out_row_stride : width;
+    const uint64_t ps = a.pos_row_stride ? a.pos_row_stride : a.axes;
+    if (width > 0x7FFFFFFFu || xs >= (1ull << 40) || os >= (1ull << 40) || ps >= (1ull << 40))
+        return fail(BL_ERR_UNSUPPORTED, "rope: rows of %llu values", (unsigned long long)width);
+    if (a.rows > 0x7FFFFFFFu) return fail(BL_ERR_UNSUPPORTED, "rope: %u rows", a.rows);
+    if (xs < width || os < width || ps < a.axes)
+        return fail(BL_ERR_INVALID, "rope: a row stride is shorter than its row");
+    const uintptr_t px = reinterpret_cast<uintptr_t>(a.x), po = reinterpret_cast<uintptr_t>(a.out);
+    if (px % esz || po % esz || (reinterpret_cast<uintptr_t>(a.positions) & 3u))
+        return fail(BL_ERR_INVALID, "rope: a buffer is not aligned to its type");
+    // In place, or apart: rows that overlap otherwise would be read after
+    // they are written. Columns of one wider row set apart are apart.
+    if (px == po) {
+        if (xs != os && a.rows > 1)
+            return fail(BL_ERR_INVALID, "rope: in place with two row strides");
+    } else if (px < po + span_bytes(a.rows, os, width, esz) &&
+               po < px + span_bytes(a.rows, xs, width, esz)) {
+        const uint64_t d = (px < po ? po - px : px - po) % (xs * esz);
+        if (xs != os || d < width * esz || d + width * esz > xs * esz)
+            return fail(BL_ERR_INVALID, "rope: x and out overlap without being the same");
+    }
+    RopeParams p{};
+    p.rows = a.rows, p.heads = static_cast<int>(a.heads), p.head_dim = static_cast<int>(a.head_dim);
+    p.pairs = static_cast<int>(pairs), p.axes = static_cast<int>(a.axes);
+    for (uint32_t i = 0; i < a.axes; ++i) p.sections[i] = static_cast<int>(a.sections[i]);
+    p.pairing = a.pairing, p.inverse = a.inverse != 0;
+    p.x = a.x, p.x_stride = static_cast<long long>(xs);
+    p.out = a.out, p.out_stride = static_cast<long long>(os);
+    p.pos = a.positions, p.pos_stride = static_cast<long long>(ps);
+    int j = 0;
+    for (uint32_t i = 0; i < a.axes; ++i)
+        for (uint32_t k = 0; k < a.sections[i]; ++k, ++j) {
+            const double f = a.freqs != nullptr ? a.freqs[j]
+                             : a.shared_ladder
+                                 ? std::pow(a.theta, -static_cast<double>(j) / static_cast<double>(pairs))
+                                 : std::pow(a.theta, -static_cast<double>(k) / a.sections[i]);
+            if (!std::isfinite(f)) return fail(BL_ERR_INVALID, "rope: frequency %d is not finite", j);
+            p.turn[j] = f / 3.14159265358979323846;
+        }
+    auto kern = a.dtype == BL_F32   ? packed::rope_kernel<float>
+                : a.dtype == BL_F16 ? packed::rope_kernel<__half>
+                                    : packed::rope_kernel<__nv_bfloat16>;
+    out->op = BL_OP_ROPE;
+    out->run = [=](cudaStream_t s) {
+        return launch_k(kern, dim3(static_cast<unsigned>(p.rows)), dim3(256), 0, s, p);
+    };
+    return BL_OK;
+}
+
+}  // namespace bl
+
+extern "C" int bl_pack(const bl_pack_args* args, void* stream) {
+    if (args == nullptr) return bl::fail(BL_ERR_INVALID, "pack: null args");
+    return bl::guarded("pack", [&] {
+        bl::Launch l;
+        const int rc = bl::prepare_pack(*args, &l);
+        return rc != BL_OK ? rc : bl::enqueue(l, static_cast<cudaStream_t>(stream));
+    });
+}
+
+extern "C" int bl_rope(const bl_rope_args* args, void* stream) {
+    if (args == nullptr) return bl::fail(BL_ERR_INVALID, "rope: null args");
+    return bl::guarded("rope", [&] {
+        bl::Launch l;
+        const int rc = bl::prepare_rope(*args, &l);
+        return rc != BL_OK ? rc : bl::enqueue(l, static_cast<cudaStream_t>(stream));
+    });
+}

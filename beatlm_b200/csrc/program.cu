@@ -294,7 +294,10 @@ bool split_dims(const bl_kernel_spec& s, uint32_t* extent, uint32_t* grain) {
         case BL_OP_GEMM: *extent = static_cast<const bl_gemm_args*>(s.args)->m; *grain = 128; return true;
         case BL_OP_LAYERNORM: *extent = static_cast<const bl_layernorm_args*>(s.args)->rows; return true;
         case BL_OP_PATCHIFY:
-        case BL_OP_ALLGATHER: return true;
+        case BL_OP_ALLGATHER:
+        case BL_OP_PACK:
+        case BL_OP_ROPE:
+        case BL_OP_MASKED_ATTENTION: return true;
         default: return false;
     }
 }
@@ -330,6 +333,11 @@ void rebind(bl_gemm_args& g, Rebind& r) {
 void rebind(bl_layernorm_args& a, Rebind& r) { r(a.x), r(a.gamma), r(a.beta), r(a.out); }
 void rebind(bl_patchify_args& a, Rebind& r) { r(a.image), r(a.a), r(a.cls), r(a.pos), r(a.x); }
 void rebind(bl_allgather_args& a, Rebind& r) { r(a.send), r(a.recv); }
+void rebind(bl_pack_args& a, Rebind& r) { r(a.grids), r(a.offsets), r(a.image), r(a.positions); }
+void rebind(bl_rope_args& a, Rebind& r) { r(a.x), r(a.positions), r(a.out); }
+void rebind(bl_masked_attention_args& a, Rebind& r) {
+    r(a.qkv), r(a.out), r(a.offsets), r(a.lengths), r(a.prefix), r(a.slopes), r(a.positions);
+}
 
 // Part [edges[i], edges[i + 1]) of spec `s` with binding set `set` (NULL =
 // as given); *moved = how many pointer arguments the set redirected.
@@ -377,6 +385,24 @@ int prepare_part(const bl_kernel_spec& s, const std::vector<uint32_t>& edges, ui
             };
             return BL_OK;
         }
+        case BL_OP_PACK: {
+            bl_pack_args a = *static_cast<const bl_pack_args*>(s.args);
+            rebind(a, r);
+            *moved = r.moved;
+            return prepare_pack(a, l);
+        }
+        case BL_OP_ROPE: {
+            bl_rope_args a = *static_cast<const bl_rope_args*>(s.args);
+            rebind(a, r);
+            *moved = r.moved;
+            return prepare_rope(a, l);
+        }
+        case BL_OP_MASKED_ATTENTION: {
+            bl_masked_attention_args a = *static_cast<const bl_masked_attention_args*>(s.args);
+            rebind(a, r);
+            *moved = r.moved;
+            return prepare_masked_attention(a, l);
+        }
         default: {
             bl_patchify_args a = *static_cast<const bl_patchify_args*>(s.args);
             rebind(a, r);
@@ -395,7 +421,7 @@ int add_spec(bl_kernels* k, const bl_kernel_spec& s, size_t index, const bl_bind
     if (!split_dims(s, &extent, &grain))
         return fail(BL_ERR_INVALID, "kernel %zu: unknown op %d", index, s.op);
     std::vector<uint32_t> edges(static_cast<size_t>(s.parts > 1 ? s.parts : 1) + 1);
-    const bool whole = s.op == BL_OP_PATCHIFY || s.op == BL_OP_ALLGATHER;
+    const bool whole = s.op == BL_OP_PATCHIFY || s.op >= BL_OP_ALLGATHER;
     const uint32_t count = whole ? 1 : bl_split_edges(extent, grain, s.parts, edges.data());
     if (whole) { edges[0] = 0; edges[1] = 1; }
     for (uint32_t i = 0; i < count; ++i) {

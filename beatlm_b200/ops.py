@@ -262,6 +262,235 @@ def patchify(image, *, stream=None, **kw):
     return kw["a_out"]
 
 
+# ------------------------------------------------------------------ packed batches
+# Images and clips of different sizes in one token buffer: their row maps,
+# rotary positions on their packed Q and K rows, and attention that masks by
+# sequence.
+
+MASK = {None: 0, "none": 0, "causal": 1, "prefix": 2}
+PAIRING = {"half": 0, "adjacent": 1, "axis_half": 2}
+
+
+def _check(what, t, dtype=None, rows=None):
+    """A CUDA tensor of `dtype` (None = any) whose last dimension is contiguous."""
+    if not t.is_cuda:
+        raise ValueError("%s: a CUDA tensor, not one on %s" % (what, t.device))
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError("%s: %s, not %s" % (what, dtype, t.dtype))
+    if t.numel() and t.stride(-1) != 1:
+        raise ValueError("%s: the last dimension is contiguous" % what)
+    if rows is not None and t.shape[0] < rows:
+        raise ValueError("%s: %d rows, %d needed" % (what, t.shape[0], rows))
+    return t
+
+
+def _launch(fn, args, tensor, stream):
+    """Calls `fn` on `tensor`'s device, whichever device is current."""
+    import torch
+    if tensor.device.index == torch.cuda.current_device():
+        N.check(fn(ctypes.byref(args), _stream_ptr(stream)))
+        return
+    with torch.cuda.device(tensor.device):
+        N.check(fn(ctypes.byref(args), _stream_ptr(stream)))
+
+
+def _same_device(what, first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError("%s: tensors on %s and %s" % (what, first.device, t.device))
+
+
+def pack_args(grids, *, offsets, image=None, positions=None, capacity=None, lead=0,
+              normalized=False):
+    """``grids``: int32 ``[images][3]`` (t, h, w); ``offsets``: int32
+    ``[images + 1]``; ``image``: int32 ``[capacity]`` or None; ``positions``:
+    f32 ``[capacity][3]`` or None. ``capacity`` defaults to the rows of
+    ``image`` or ``positions``."""
+    import torch
+    _check("pack: grids", grids, torch.int32)
+    if grids.dim() != 2 or grids.shape[1] != 3 or not grids.is_contiguous():
+        raise ValueError("pack: grids are contiguous [images][3], not %s" % (tuple(grids.shape),))
+    n = grids.shape[0]
+    _check("pack: offsets", offsets, torch.int32, n + 1)
+    if capacity is None:
+        have = image if image is not None else positions
+        if have is None:
+            raise ValueError("pack: a capacity, an image map or positions")
+        capacity = have.shape[0]
+    if image is not None:
+        _check("pack: image", image, torch.int32, capacity)
+    if positions is not None:
+        _check("pack: positions", positions, torch.float32, capacity)
+        if positions.dim() != 2 or positions.shape[1] != 3 or not positions.is_contiguous():
+            raise ValueError("pack: positions are contiguous [capacity][3]")
+    if not 0 <= lead < 2 ** 31 or not 0 <= capacity < 2 ** 31:
+        raise ValueError("pack: %d lead rows, %d rows" % (lead, capacity))
+    _same_device("pack", grids, offsets, image, positions)
+    return N.PackArgs(images=n, capacity=capacity, lead=lead, normalized=1 if normalized else 0,
+                      grids=grids.data_ptr(), offsets=offsets.data_ptr(), image=_ptr(image),
+                      positions=_ptr(positions))
+
+
+def pack(grids, *, offsets, stream=None, **kw):
+    """Row maps of a packed batch, built on the GPU (``bl_pack``): each image's
+    first row, each row's image and its patch's (t, y, x). Returns
+    ``offsets``."""
+    a = pack_args(grids, offsets=offsets, **kw)
+    _launch(N.lib().bl_pack, a, grids, stream)
+    return offsets
+
+
+def rope_args(x, positions, *, sections, theta=100.0, freqs=None, shared=False, pairing="half",
+              inverse=False, heads=None, head_dim=None, dtype=None, out=None):
+    """``x``: ``[rows][heads][head_dim]``, or ``[rows][width]`` with ``heads``
+    and ``head_dim`` (the leading heads of packed rows; an int16 container
+    takes its type from ``dtype``). ``positions``: f32 ``[rows][axes or
+    more]``, the axes its first columns. ``sections``: the pairs of each axis.
+    ``freqs``: the host's own radians a unit of position, one a pair."""
+    import torch
+    _check("rope: x", x)
+    _check("rope: positions", positions, torch.float32)
+    out = x if out is None else _check("rope: out", out)
+    if x.dim() == 3:
+        if (heads or x.shape[1]) != x.shape[1] or (head_dim or x.shape[2]) != x.shape[2]:
+            raise ValueError("rope: %s heads of %s in %s" % (heads, head_dim, tuple(x.shape)))
+        heads, head_dim = x.shape[1], x.shape[2]
+    if x.dim() not in (2, 3) or not heads or not head_dim:
+        raise ValueError("rope: x is [rows][heads][head_dim], or [rows][width] with both given")
+    rows = x.shape[0]
+    for what, t in (("x", x), ("out", out)):
+        if t.dim() == 3 and t.shape[1] > 1 and t.stride(1) != head_dim:
+            raise ValueError("rope: the heads of a row of %s are neighbours" % what)
+        if t.shape[0] != rows or (t.dim() == 3 and t.shape != x.shape) or \
+                t[0:1].numel() < heads * head_dim or t.dtype != x.dtype:
+            raise ValueError("rope: %s is %s of %s" % (what, tuple(t.shape), t.dtype))
+    axes = len(sections)
+    if not 1 <= axes <= 3 or positions.dim() != 2 or positions.shape[0] < rows or \
+            positions.shape[1] < axes:
+        raise ValueError("rope: positions %s for %d rows and %d axes (1 to 3)"
+                         % (tuple(positions.shape), rows, axes))
+    if any(int(n) < 1 for n in sections):
+        raise ValueError("rope: sections %s" % (tuple(sections),))
+    if dtype is None and not x.dtype.is_floating_point:
+        raise ValueError("rope: the dtype of a %s container" % x.dtype)
+    if dtype is not None and (x.element_size() != (4 if dtype == "f32" else 2) or (
+            x.dtype.is_floating_point and _dt(x) != _TD[dtype])):
+        raise ValueError("rope: %s values in a tensor of %s" % (dtype, x.dtype))
+    _same_device("rope", x, positions, out)
+    a = N.RopeArgs(rows=rows, heads=heads, head_dim=head_dim, axes=axes, pairing=PAIRING[pairing],
+                   shared_ladder=1 if shared else 0, inverse=1 if inverse else 0,
+                   dtype=_dt(x) if dtype is None else _TD[dtype], theta=theta, x=x.data_ptr(),
+                   x_row_stride=x.stride(0) if rows > 1 else 0, positions=positions.data_ptr(),
+                   pos_row_stride=positions.stride(0) if rows > 1 else 0, out=out.data_ptr(),
+                   out_row_stride=out.stride(0) if rows > 1 else 0)
+    a.sections[:axes] = [int(n) for n in sections]
+    if freqs is not None:
+        if len(freqs) != sum(int(n) for n in sections):
+            raise ValueError("rope: %d frequencies for sections %s" % (len(freqs), tuple(sections)))
+        a._freqs = (ctypes.c_double * len(freqs))(*[float(f) for f in freqs])
+        a.freqs = ctypes.addressof(a._freqs)
+    return a
+
+
+def rope(x, positions, *, sections, out=None, stream=None, **kw):
+    """Rotary positions with 1 to 3 axes (``bl_rope``) on the heads of ``x``,
+    in place or into ``out``; ``inverse=True`` turns back (the gradient)."""
+    out = x if out is None else out
+    a = rope_args(x, positions, sections=sections, out=out, **kw)
+    if a.rows:
+        _launch(N.lib().bl_rope, a, x, stream)
+    return out
+
+
+def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets=None,
+                          lengths=None, last_rows=0, qk_dtype="f16", out_dtype=None, scale=None,
+                          mask=None, prefix=None, cap=None, slopes=None, positions=None,
+                          key_splits=0):
+    """``qkv``: 16-bit ``[rows][(heads + 2 kv_heads) * 64]`` (or
+    ``[rows][heads + 2 kv_heads][64]``) packed rows. ``offsets`` (int32
+    ``[batch + 1]``): packed sequences; otherwise ``batch`` (default: as many
+    as ``lengths`` has, else 1) equal parts of the rows, ``lengths`` (int32
+    ``[batch]``) of each in use. ``out``: ``[rows][heads * 64]``. ``prefix``:
+    int32 ``[batch]``; ``slopes``: f32 ``[heads]``; ``positions``: f32
+    ``[rows][1 to 3 axes]``."""
+    import torch
+    if head_rows := (qkv.dim() == 3):
+        if qkv.shape[2] != 64 or (qkv.shape[1] > 1 and qkv.stride(1) != 64):
+            raise ValueError("masked attention: qkv rows of neighbouring heads of 64, not %s"
+                             % (tuple(qkv.shape),))
+    _check("masked attention: qkv", qkv)
+    _check("masked attention: out", out)
+    kv = heads if kv_heads is None else kv_heads
+    rows, width = qkv.shape[0], qkv.shape[1] * (64 if head_rows else 1)
+    if qkv.element_size() != 2 or qkv.dim() not in (2, 3) or heads < 1 or kv < 1 or \
+            width < (heads + 2 * kv) * 64:
+        raise ValueError("masked attention: qkv is %s of %s for %d heads and %d K/V heads"
+                         % (tuple(qkv.shape), qkv.dtype, heads, kv))
+    if out.dim() != 2 or out.shape[0] < rows or out.shape[1] < heads * 64:
+        raise ValueError("masked attention: out is %s for %d rows" % (tuple(out.shape), rows))
+    if offsets is not None:
+        _check("masked attention: offsets", offsets, torch.int32)
+        if batch is None:
+            batch = offsets.numel() - 1
+        if offsets.numel() < batch + 1 or not offsets.is_contiguous():
+            raise ValueError("masked attention: %d offsets for %d sequences"
+                             % (offsets.numel(), batch))
+        tokens = rows
+    else:
+        if batch is None:
+            batch = 1 if lengths is None else lengths.numel()
+        if batch < 1 or rows % batch:
+            raise ValueError("masked attention: %d rows in %d equal parts" % (rows, batch))
+        tokens = rows // batch
+    for what, t, n, dt in (("lengths", lengths, batch, torch.int32),
+                           ("prefix", prefix, batch, torch.int32),
+                           ("slopes", slopes, heads, torch.float32)):
+        if t is not None and (_check("masked attention: " + what, t, dt).numel() < n
+                              or not t.is_contiguous()):
+            raise ValueError("masked attention: %d %s, %d needed" % (t.numel(), what, n))
+    if positions is not None:
+        _check("masked attention: positions", positions, torch.float32, rows)
+        if positions.dim() != 2 or not 1 <= positions.shape[1] <= 3:
+            raise ValueError("masked attention: positions are [rows][1 to 3], not %s"
+                             % (tuple(positions.shape),))
+    if last_rows < 0 or (cap is not None and not cap > 0):
+        raise ValueError("masked attention: last_rows %s, cap %s" % (last_rows, cap))
+    _same_device("masked attention", qkv, out, offsets, lengths, prefix, slopes, positions)
+    many = rows > 1
+    return N.MaskedAttentionArgs(
+        batch=batch, tokens=tokens, heads=heads, kv_heads=kv, head_dim=64,
+        last_rows=min(last_rows, 2 ** 31 - 1), scale=0.125 if scale is None else scale,
+        cap=0.0 if cap is None else cap, mask=MASK[mask], qk_dtype=_TD[qk_dtype],
+        v_dtype=N.BL_F16, out_dtype=_dt(out) if out_dtype is None else _TD[out_dtype],
+        qkv=qkv.data_ptr(), qkv_row_stride=qkv.stride(0) if many else 0, out=out.data_ptr(),
+        out_row_stride=out.stride(0) if many else 0, offsets=_ptr(offsets), lengths=_ptr(lengths),
+        prefix=_ptr(prefix), slopes=_ptr(slopes), positions=_ptr(positions),
+        pos_row_stride=positions.stride(0) if positions is not None and many else 0,
+        pos_axes=0 if positions is None else positions.shape[1], key_splits=key_splits)
+
+
+def masked_attention(qkv, *, heads, out=None, out_dtype=None, stream=None, **kw):
+    """Attention over packed or padded sequences with capped scores, a bias of
+    distance and document, causal or prefix masks (``bl_masked_attention``);
+    ``last_rows`` computes the newest rows of every sequence alone. Without
+    ``out`` a zero-filled ``[rows][heads * 64]`` of ``out_dtype`` (default
+    "f16") is made; rows that are not computed are left as they were."""
+    import torch
+    if out is None:
+        tdt = {"f32": torch.float32, "f16": torch.float16,
+               "bf16": torch.bfloat16}[out_dtype or "f16"]
+        out = torch.zeros((qkv.shape[0], heads * 64), dtype=tdt, device=qkv.device)
+        out_dtype = None
+    elif out.dtype.is_floating_point:
+        if out_dtype is not None and _dt(out) != _TD[out_dtype]:
+            raise ValueError("masked attention: out is %s, not %s" % (out.dtype, out_dtype))
+        out_dtype = None
+    a = masked_attention_args(qkv, heads=heads, out=out, out_dtype=out_dtype, **kw)
+    if a.batch and a.tokens:
+        _launch(N.lib().bl_masked_attention, a, qkv, stream)
+    return out
+
+
 # ------------------------------------------------------------------ DPT decoder
 # The reference's Conv2d3x3 / Conv2d1x1 / ConvTranspose2d / ResizeBilinear main
 # ops (crates/beatlm-core/src/kernel.rs:265-319, wgsl.rs:387-514; CPU

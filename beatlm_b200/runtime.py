@@ -14,9 +14,11 @@ from . import _native as N
 from .ops import _stream_ptr
 
 OP_ATTENTION, OP_GEMM, OP_LAYERNORM, OP_PATCHIFY, OP_ALLGATHER = 1, 2, 3, 4, 5
+OP_PACK, OP_ROPE, OP_MASKED_ATTENTION = 6, 7, 8
 _OP_OF = {N.AttentionArgs: OP_ATTENTION, N.GemmArgs: OP_GEMM,
           N.LayerNormArgs: OP_LAYERNORM, N.PatchifyArgs: OP_PATCHIFY,
-          N.AllGatherArgs: OP_ALLGATHER}
+          N.AllGatherArgs: OP_ALLGATHER, N.PackArgs: OP_PACK, N.RopeArgs: OP_ROPE,
+          N.MaskedAttentionArgs: OP_MASKED_ATTENTION}
 
 
 def hold(stream, microseconds: int):

@@ -495,6 +495,147 @@ typedef struct bl_patchify_args {
 
 int bl_patchify(const bl_patchify_args* args, void* stream);
 
+/* ------------------------------------------------------------ packed batches */
+
+/*
+ * Row maps of a packed batch, built on the GPU: images and clips of different
+ * sizes, one after the other in one token buffer of `capacity` rows. The
+ * reference runs one image size per graph (TokensToMap and the position Add
+ * are compiled for it, crates/beatlm-core/src/kernel.rs:689-720); a host that
+ * batches requests of many sizes needs the rows of each and their positions,
+ * and reading the sizes back to the CPU would stall its frame loop.
+ *
+ * grids[i] = (t, h, w), int32: image i takes n_i = lead + t h w rows (`lead`
+ * class or register tokens first, then its patches, t outermost), or none when
+ * one of the three is not positive. Written:
+ *   offsets[0..images]   int32: offsets[0] = 0, offsets[i + 1] = offsets[i] + n_i;
+ *   image[0..capacity)   int32 (NULL = not wanted): the row's image, -1 behind
+ *                        the last;
+ *   positions[capacity][3]  f32 (NULL = not wanted): (t, y, x) of a patch row,
+ *                        or with `normalized` (2 c + 1 - n) / n of each
+ *                        coordinate c of n, the patch centres spread over
+ *                        (-1, 1); zeros for the lead rows (which bl_rope then
+ *                        leaves as they are) and behind the last image.
+ * Rows past `capacity` are cut off (their offsets are `capacity`) and recorded
+ * in the device status word (0x50). Enqueues on `stream`; allocates nothing
+ * and waits for nothing on the host.
+ */
+typedef struct bl_pack_args {
+    uint32_t images;
+    uint32_t capacity;   /* rows of the token buffer, below 2^31 */
+    uint32_t lead;
+    uint32_t normalized;
+    const int32_t* grids;
+    int32_t* offsets;
+    int32_t* image;
+    float* positions;
+} bl_pack_args;
+int bl_pack(const bl_pack_args* args, void* stream);
+
+/*
+ * Rotary positions with one to three axes (time, height, width) on the heads
+ * of packed rows: `heads` neighbouring heads of head_dim values from x on, row
+ * r at x + r * x_row_stride, so one call turns the Q and the K section of a
+ * packed Q|K|V row (heads = q heads + k heads). No counterpart in the
+ * reference, whose models add learned positions to the embedding
+ * (kernel.rs:689-701).
+ *
+ * Axis a owns sections[a] neighbouring pairs; pair p of axis a turns by
+ *   angle = positions[r][a] * freq[p]
+ *   lo' = lo cos - hi sin, hi' = hi cos + lo sin   (inverse: sin negated)
+ * with freq[p] = theta^(-k / sections[a]) for the axis's k-th pair, with
+ * shared_ladder theta^(-p / pairs) over all pairs, or the host's own `freqs`
+ * (64-bit, one a pair, read during the call). `pairing` says which two values
+ * of the head a pair is: BL_ROPE_HALF (p, p + pairs), BL_ROPE_ADJACENT
+ * (2 p, 2 p + 1), or BL_ROPE_AXIS_HALF (halves within each axis's block of
+ * 2 sections[a] values). Values past 2 * pairs do not turn. The inverse is the
+ * gradient of the rotation as well (it is orthogonal).
+ *
+ * Angles are formed in 64 bits, the rotation in f32, each result rounded once.
+ * out may be x (with its stride) or apart from it. Enqueues on `stream`;
+ * allocates nothing.
+ */
+enum { BL_ROPE_HALF = 0, BL_ROPE_ADJACENT = 1, BL_ROPE_AXIS_HALF = 2 };
+enum { BL_ROPE_MAX_PAIRS = 128 };
+typedef struct bl_rope_args {
+    uint32_t rows, heads, head_dim;
+    uint32_t axes;
+    uint32_t sections[3];
+    int32_t pairing;
+    uint32_t shared_ladder;
+    uint32_t inverse;
+    int32_t dtype;            /* of x and out: BL_F32, BL_F16 or BL_BF16 */
+    double theta;
+    const double* freqs;      /* host memory; NULL = from theta */
+    const void* x;
+    uint64_t x_row_stride;    /* elements; 0 = heads * head_dim */
+    const float* positions;   /* device: [rows][axes] */
+    uint64_t pos_row_stride;  /* 0 = axes */
+    void* out;
+    uint64_t out_row_stride;  /* 0 = heads * head_dim */
+} bl_rope_args;
+int bl_rope(const bl_rope_args* args, void* stream);
+
+/*
+ * Attention over sequences with capped scores, a bias of distance and masks,
+ * beside bl_attention (which runs one dense sequence length per batch):
+ *   s_ij = scale q_i . k_j;  cap > 0: s_ij = cap tanh(s_ij / cap);
+ *   slopes: s_ij -= slopes[head] * dist(i, j), dist = |i - j|, or with
+ *   positions the Euclidean distance of the rows' pos_axes coordinates;
+ *   o_i = sum_j softmax_j(s_ij) v_j over the keys j that row i sees:
+ *   those of its own sequence, and with BL_MASK_CAUSAL j <= i, with
+ *   BL_MASK_PREFIX j <= i or j < prefix[sequence] (places within the
+ *   sequence; the prefix sees itself whole).
+ *
+ * Rows are packed per token as in bl_attention, [heads + 2 kv_heads][64]
+ * (Q heads, K heads, V heads; q head h reads K/V head h / (heads / kv_heads);
+ * kv_heads 0 = heads), Q and K f16 or bf16, V f16. Two forms of a batch:
+ *   packed (offsets != NULL): `batch` sequences in a buffer of `tokens` rows,
+ *     sequence s in rows [offsets[s], offsets[s + 1]) (bl_pack's offsets);
+ *   padded: `batch` sequences of `tokens` rows each, of which the first
+ *     lengths[s] are in use (NULL = all).
+ * Offsets and lengths are device memory, read by the kernel and clamped to the
+ * buffer, so a recorded launch follows them as they change. A sequence may be
+ * empty. last_rows > 0 computes only the last rows of every sequence (the
+ * newest tokens of a stream over the rows it has kept); output rows have the
+ * places of their query rows, and rows outside (not asked for, behind a
+ * sequence) are left as they were. Values behind a sequence's end, NaN or
+ * infinite included, never reach a result; within a sequence a value that is
+ * not finite may reach every row of it.
+ *
+ * Scores, statistics and sums are f32; with more than a few query rows per K/V
+ * head the probabilities are rounded to f16 for the tensor cores (as in
+ * bl_attention). key_splits: how many CTAs share a tile's keys (a cluster,
+ * combined on chip): 0 = automatic, at most 8. head_dim must be 64; qkv and out
+ * 16-byte aligned with strides of 16-byte multiples. Enqueues on `stream`;
+ * allocates nothing; no workspace, and the same bits in every run.
+ */
+enum { BL_MASK_NONE = 0, BL_MASK_CAUSAL = 1, BL_MASK_PREFIX = 2 };
+typedef struct bl_masked_attention_args {
+    uint32_t batch, tokens;
+    uint32_t heads, kv_heads, head_dim;
+    uint32_t last_rows;
+    float scale;
+    float cap;               /* 0 = none */
+    int32_t mask;            /* BL_MASK_* */
+    int32_t qk_dtype;
+    int32_t v_dtype;         /* BL_F16 */
+    int32_t out_dtype;
+    const void* qkv;
+    uint64_t qkv_row_stride; /* 0 = (heads + 2 kv_heads) * 64 */
+    void* out;
+    uint64_t out_row_stride; /* 0 = heads * 64 */
+    const int32_t* offsets;  /* device [batch + 1], or NULL */
+    const int32_t* lengths;  /* device [batch], or NULL */
+    const int32_t* prefix;   /* device [batch]; BL_MASK_PREFIX only */
+    const float* slopes;     /* device [heads], or NULL */
+    const float* positions;  /* device [rows of qkv][pos_axes], or NULL */
+    uint64_t pos_row_stride; /* 0 = pos_axes */
+    uint32_t pos_axes;       /* 1 to 3 */
+    uint32_t key_splits;
+} bl_masked_attention_args;
+int bl_masked_attention(const bl_masked_attention_args* args, void* stream);
+
 /* ------------------------------------------------------------------ splitting */
 
 /*
@@ -514,7 +655,7 @@ uint32_t bl_parts_within(uint64_t duration_us, uint64_t bound_us, uint32_t max_p
 /* ------------------------------------------------------------------ kernels */
 
 enum { BL_OP_ATTENTION = 1, BL_OP_GEMM = 2, BL_OP_LAYERNORM = 3, BL_OP_PATCHIFY = 4,
-       BL_OP_ALLGATHER = 5 };
+       BL_OP_ALLGATHER = 5, BL_OP_PACK = 6, BL_OP_ROPE = 7, BL_OP_MASKED_ATTENTION = 8 };
 
 /* The arguments of a BL_OP_ALLGATHER kernel spec: bl_comm_all_gather encoded
  * like a kernel (recorded into a program, replayed in its CUDA graph). */
@@ -529,8 +670,8 @@ typedef struct bl_allgather_args {
  * read during bl_kernels_create only), a label, and the number of row parts
  * it runs as (0 or 1 = whole). Split dimensions and grains: attention query
  * rows in 128-row tiles (every frame of the batch), GEMM output rows in
- * 128-row tiles, LayerNorm rows one by one; patchify and all-gather are
- * never split. */
+ * 128-row tiles, LayerNorm rows one by one; patchify, all-gather and the
+ * packed-batch kernels are never split. */
 typedef struct bl_kernel_spec {
     int32_t op;
     const void* args;

@@ -1,0 +1,126 @@
+"""Refusals of the packed-batch operators: every malformed argument is turned
+away on the host, before anything is launched (no GPU needed)."""
+import ctypes
+
+import pytest
+
+from beatlm_b200 import _native as N
+
+A = 1 << 20  # an aligned address; nothing is launched, so nothing reads it
+
+
+def _call(fn, a):
+    N.check(fn(ctypes.byref(a), None))
+
+
+def _pack(**kw):
+    base = dict(images=3, capacity=100, lead=1, grids=A, offsets=2 * A, image=3 * A,
+                positions=4 * A)
+    base.update(kw)
+    return N.PackArgs(**base)
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(images=0), "no images"), (dict(capacity=0), "no rows"), (dict(grids=None), "null"),
+    (dict(offsets=None), "null"), (dict(capacity=1 << 31), "32-bit"),
+    (dict(lead=1 << 31), "32-bit"), (dict(images=0x7FFFFFFF), "32-bit"),
+    (dict(offsets=2 * A + 2), "aligned"), (dict(positions=4 * A + 1), "aligned")])
+def test_pack_refuses(kw, why):
+    with pytest.raises(N.BackendError, match=why):
+        _call(N.lib().bl_pack, _pack(**kw))
+
+
+def _rope(sections=(16, 16), **kw):
+    base = dict(rows=10, heads=4, head_dim=64, axes=2, pairing=0, dtype=N.BL_BF16, theta=100.0,
+                x=A, positions=2 * A, out=A)
+    base.update(kw)
+    a = N.RopeArgs(**base)
+    for i, n in enumerate(sections):
+        a.sections[i] = n
+    return a
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(rows=0), "zero"), (dict(heads=0), "zero"), (dict(axes=0), "axes"),
+    (dict(axes=4), "axes"), (dict(sections=(16, 0)), "no pairs"),
+    (dict(sections=(16, 17)), "33 pairs"), (dict(sections=(0xFFFFFFFF, 1)), "pairs in a head"),
+    (dict(sections=(100, 100), head_dim=512), "at most"), (dict(pairing=3), "pairing"),
+    (dict(dtype=3), "dtype"), (dict(theta=0.0), "theta"), (dict(theta=float("inf")), "theta"),
+    (dict(theta=float("nan")), "theta"), (dict(x=None), "null"), (dict(out=None), "null"),
+    (dict(positions=None), "null"), (dict(x_row_stride=255), "shorter"),
+    (dict(out_row_stride=255), "shorter"), (dict(pos_row_stride=1), "shorter"),
+    (dict(x=A + 1), "aligned"), (dict(positions=2 * A + 2), "aligned"),
+    (dict(out_row_stride=512), "in place"), (dict(out=A + 64), "overlap"),
+    (dict(out=A + 512, x_row_stride=512, out_row_stride=256), "overlap"),
+    (dict(out=A + 256, x_row_stride=512, out_row_stride=512), "overlap"),
+    (dict(heads=1 << 26, head_dim=64, x_row_stride=0), "values"),
+    (dict(rows=1 << 31), "rows")])
+def test_rope_refuses(kw, why):
+    with pytest.raises(N.BackendError, match=why):
+        _call(N.lib().bl_rope, _rope(**kw))
+
+
+def test_rope_refuses_frequencies_that_are_not_finite():
+    f = (ctypes.c_double * 32)(*([1.0] * 31 + [float("nan")]))
+    with pytest.raises(N.BackendError, match="frequency 31"):
+        _call(N.lib().bl_rope, _rope(freqs=ctypes.addressof(f)))
+
+
+def _attn(**kw):
+    base = dict(batch=2, tokens=64, heads=4, kv_heads=2, head_dim=64, scale=0.125,
+                qk_dtype=N.BL_F16, v_dtype=N.BL_F16, out_dtype=N.BL_BF16, qkv=A, out=2 * A)
+    base.update(kw)
+    return N.MaskedAttentionArgs(**base)
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(head_dim=32), "head_dim"), (dict(batch=0), "zero"), (dict(tokens=0), "zero"),
+    (dict(heads=0), "zero"), (dict(kv_heads=3), "K/V heads"), (dict(heads=70000), "heads"),
+    (dict(offsets=4 * A, lengths=5 * A), "packed"), (dict(batch=1 << 16, tokens=1 << 16), "rows"),
+    (dict(qk_dtype=N.BL_F32), "Q/K dtype"), (dict(v_dtype=N.BL_BF16), "V dtype"),
+    (dict(out_dtype=7), "out dtype"), (dict(scale=0.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(cap=-1.0), "cap"), (dict(cap=float("inf")), "cap"),
+    (dict(cap=float("nan")), "cap"), (dict(mask=3), "mask 3"), (dict(mask=2), "prefix"),
+    (dict(prefix=4 * A), "prefix"), (dict(positions=4 * A, pos_axes=2), "slopes"),
+    (dict(positions=4 * A, slopes=5 * A), "position axes"),
+    (dict(positions=4 * A, slopes=5 * A, pos_axes=4), "position axes"),
+    (dict(positions=4 * A, slopes=5 * A, pos_axes=2, pos_row_stride=1), "shorter"),
+    (dict(key_splits=9), "key splits"), (dict(qkv=None), "null"), (dict(out=None), "null"),
+    (dict(qkv_row_stride=504), "stride"), (dict(qkv_row_stride=516), "stride"),
+    (dict(qkv=A + 8), "alignment"), (dict(out=2 * A + 8), "alignment"),
+    (dict(out_row_stride=255), "output"), (dict(out_row_stride=260), "output"),
+    (dict(lengths=4 * A + 2), "4-byte")])
+def test_masked_attention_refuses(kw, why):
+    with pytest.raises(N.BackendError, match=why):
+        _call(N.lib().bl_masked_attention, _attn(**kw))
+
+
+def test_null_arguments():
+    for f in ("bl_pack", "bl_rope", "bl_masked_attention"):
+        with pytest.raises(N.BackendError, match="null args"):
+            N.check(getattr(N.lib(), f)(None, None))
+
+
+def test_programs_take_the_packed_batch_kernels():
+    """Each is a kernel of its own kind that is never split; a program refuses
+    what the call refuses."""
+    from beatlm_b200 import runtime as R
+    for a in (_pack(), _rope(), _attn()):
+        assert R.max_parts(R.Spec(a, "k", parts=4)) == 1
+    for a, why in ((_pack(images=0), "no images"), (_rope(pairing=9), "pairing"),
+                   (_attn(mask=9), "mask 9")):
+        with pytest.raises(N.BackendError, match=why):
+            R.Kernels([R.Spec(a, "k")])
+
+
+def test_python_calls_refuse_cpu_tensors():
+    import torch
+    from beatlm_b200 import ops
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.pack(torch.ones((2, 3), dtype=torch.int32), offsets=torch.zeros(3, dtype=torch.int32),
+                 capacity=4)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.rope(torch.zeros((2, 1, 64)), torch.zeros((2, 2)), sections=(16, 16))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.masked_attention(torch.zeros((2, 3, 64), dtype=torch.int16), heads=1,
+                             out=torch.zeros((2, 64)))
