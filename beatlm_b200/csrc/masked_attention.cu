@@ -282,6 +282,550 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(const Params p, int b
     if (p.splits > 1) cluster_sync();  // no CTA leaves while its partials are read
 }
 
+// ------------------------------------------------------------------ tiles
+//
+// One CTA computes 128 query rows of one head over a range of 64-key tiles on
+// the tensor cores; two CTAs share an SM (256 threads of at most 128
+// registers, half the TMEM each), so one's exponentials run beside the
+// other's waits and a tile's set-up and end are hidden by its neighbour.
+// Warps:
+//   0     TMA producer: the Q tile once, then K and V tiles into a ring.
+//   1     MMA issuer: S = Q K^T (M 128, N 64, K 64) into one of three TMEM
+//         buffers, O += P V (P from TMEM, f16). S of tile i + 3 follows
+//         PV(i) in the tensor pipe, whose buffer it takes.
+//   2     finds the CTA's sequence among the packed ones.
+//   4..7  softmax, one thread a query row (TMEM lane).
+// Tiles start at their sequence's first row, so a key tile holds keys of one
+// sequence, and past its end only rows that no query sees: their scores are
+// replaced by -inf and their V rows zeroed in shared memory before the
+// product, since 0 * NaN from another sequence's rows would reach O.
+constexpr int BM = 128;
+constexpr int BN = 64;
+constexpr int STAGES = 5;
+constexpr int SBUFS = 3;
+constexpr int kTileThreads = 256;
+constexpr uint32_t kQBytes = BM * HD * 2;
+constexpr uint32_t kKvBytes = BN * HD * 2;
+constexpr uint32_t kTmemCols = 256;
+constexpr uint32_t kColO = SBUFS * BN;
+static_assert(kColO + HD <= kTmemCols, "TMEM columns");
+// The running maximum may trail the true one by this much (log2 units) before
+// O is rescaled: P stays below 2^8, well inside f16.
+constexpr float kRescaleThreshold = 8.0f;
+
+struct TileTail {
+    uint64_t q_full;
+    uint64_t kv_full[STAGES];
+    uint64_t kv_empty[STAGES];
+    uint64_t s_full[SBUFS];  // by S buffer: at most one phase ahead, as S(i + 3) waits for P(i)
+    uint64_t p_full[SBUFS];
+    // by parity of the key tile: when the softmax of tile i asks for PV(i - 1),
+    // PV(i - 3) is done (S(i) followed it), so the parity names one phase
+    uint64_t o_done[2];
+    uint64_t o_final;
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort;
+    // this CTA's work, found once
+    int seq;        // -1: none
+    int q0, rows;   // first query row within the sequence, rows of the tile
+    int keys;       // keys that some row of the tile sees
+    int t0, n;      // its key tiles
+    float kpos[4][3][BN];  // each softmax warp's copy of a key tile's positions
+};
+constexpr size_t kTileSmem = 1024 + kQBytes + 2 * STAGES * kKvBytes + sizeof(TileTail);
+static_assert(2 * (kTileSmem + 1024) <= 233472, "two CTAs an SM");
+
+// The sequence and tile of tile `index` of the packed batch: a warp walks the
+// offsets 256 sequences at a time, eight a lane. tile = -1 behind the last.
+__device__ __forceinline__ void find_tile(const Params& p, int index, int& seq, int& tile) {
+    const int lane = lane_id();
+    seq = -1, tile = 0;
+    long long total = 0;
+    for (int base = 0; base < p.batch; base += 256) {
+        int count[8], mine = 0;
+        const int first = base + 8 * lane;
+        int prev = p.offsets[min(first, p.batch)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int next = p.offsets[min(first + i + 1, p.batch)];
+            const int b = min(max(prev, 0), p.tokens), e = min(max(next, b), p.tokens);
+            count[i] = first + i < p.batch ? (e - b + BM - 1) / BM : 0;
+            mine += count[i];
+            prev = next;
+        }
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        const unsigned past = __ballot_sync(0xFFFFFFFFu, total + upto > index);
+        if (past != 0) {
+            const int owner = __ffs(past) - 1;
+            int left = static_cast<int>(index - total) - (upto - mine), s = first;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (s == first + i && left >= count[i]) left -= count[i], ++s;
+            seq = min(__shfl_sync(0xFFFFFFFFu, s, owner), p.batch - 1);
+            tile = max(__shfl_sync(0xFFFFFFFFu, left, owner), 0);
+            return;
+        }
+        total += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+}
+
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float sqrt_approx(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void store4(void* out, long long at, int dt, const float4& v) {
+    if (dt == BL_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
+    } else {
+        const uint2 w = dt == BL_F16 ? make_uint2(pack_f16x2(v.x, v.y), pack_f16x2(v.z, v.w))
+                                     : make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = w;
+    }
+}
+__device__ __forceinline__ void store8(void* out, long long at, int dt, const float* v) {
+    if (dt == BL_F32) {
+        store4(out, at, dt, make_float4(v[0], v[1], v[2], v[3]));
+        store4(out, at + 4, dt, make_float4(v[4], v[5], v[6], v[7]));
+    } else {
+        const uint4 w = dt == BL_F16
+            ? make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]),
+                         pack_f16x2(v[6], v[7]))
+            : make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                         pack_bf16x2(v[6], v[7]));
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = w;
+    }
+}
+
+enum { BIAS_NONE = 0, BIAS_INDEX = 1, BIAS_PLANE = 2, BIAS_SPACE = 3 };
+
+template <bool kCap, int kBias>
+__global__ void __launch_bounds__(kTileThreads, 2)
+    tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv,
+                const __grid_constant__ Params p, int bf16) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* sQ = smem;
+    uint8_t* sK = smem + kQBytes;                       // stage s at + s * kKvBytes
+    uint8_t* sV = sK + STAGES * kKvBytes;
+    TileTail* tail = reinterpret_cast<TileTail*>(sV + STAGES * kKvBytes);
+    volatile int* abort = &tail->abort;
+    const int warp = warp_id(), lane = lane_id();
+    const int head = blockIdx.y, kvh = head / p.group;
+    constexpr unsigned kFull = 0xFFFFFFFFu;
+
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&tail->q_full), 1);
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&tail->kv_full[s]), 1);
+            mbar_init(smem_u32(&tail->kv_empty[s]), 1);
+        }
+        for (int s = 0; s < SBUFS; ++s) {
+            mbar_init(smem_u32(&tail->s_full[s]), 1);
+            mbar_init(smem_u32(&tail->p_full[s]), BM);
+        }
+        mbar_init(smem_u32(&tail->o_done[0]), 1);
+        mbar_init(smem_u32(&tail->o_done[1]), 1);
+        mbar_init(smem_u32(&tail->o_final), 1);
+        mbar_init(smem_u32(&tail->drain), 1);
+        tail->abort = 0;
+        fence_barrier_init();
+        fence_proxy_async_smem();
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_kv);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tail->tmem_base), kTmemCols);
+        tmem_relinquish();
+    }
+    pdl_trigger();
+    pdl_wait();
+    if (warp == 2) {
+        const int unit = static_cast<int>(blockIdx.x) / p.splits;
+        const int split = static_cast<int>(blockIdx.x) % p.splits;
+        int seq, tile;
+        if (p.chunks > 0) {
+            seq = unit / p.chunks, tile = unit % p.chunks;
+        } else {
+            find_tile(p, unit, seq, tile);
+        }
+        if (seq >= 0) {
+            const Span q = span_of(p, seq);
+            const int tiles = (q.len - q.first + BM - 1) / BM;
+            if (tile >= tiles) {
+                seq = -1;
+            } else {
+                // with a causal mask the last rows see most: they start first
+                if (p.mask != BL_MASK_NONE) tile = tiles - 1 - tile;
+                const int q0 = q.first + tile * BM;
+                const int rows = min(q.len - q0, BM);
+                const int keys = visible(p, q, q0 + rows - 1);
+                const int nt = (keys + BN - 1) / BN;
+                const int t0 = static_cast<int>(1ll * nt * split / p.splits);
+                if (lane == 0) {
+                    tail->q0 = q0, tail->rows = rows, tail->keys = keys;
+                    tail->t0 = t0;
+                    tail->n = static_cast<int>(1ll * nt * (split + 1) / p.splits) - t0;
+                }
+            }
+        }
+        if (lane == 0) tail->seq = seq;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tail->tmem_base;
+    const int seq = tail->seq;
+    if (seq < 0) {  // no such tile (the same for every CTA of a cluster)
+        if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+        return;
+    }
+    const int t0 = tail->t0, n = tail->n;
+
+    if (warp == 0) {
+        // ------------------------------------------------------ producer
+        const Span q = span_of(p, seq);
+        const int row0 = static_cast<int>(q.begin);
+        const uint32_t b_q = smem_u32(&tail->q_full);
+        if (lane == 0 && n > 0) {
+            mbar_arrive_expect_tx(b_q, kQBytes);
+            tma_load_2d(smem_u32(sQ), &tm_q, head * HD, row0 + tail->q0, b_q);
+        }
+        int loaded = 0;
+        for (int i = 0; i < n; ++i) {
+            const int s = i % STAGES, r = i / STAGES;
+            bool w = true;
+            if (lane == 0 && r > 0)
+                w = mbar_wait(smem_u32(&tail->kv_empty[s]), (r - 1) & 1, abort, p.status,
+                              ST_TIMEOUT_TMA, i);
+            if (!__all_sync(kFull, w)) break;
+            const uint32_t bar = smem_u32(&tail->kv_full[s]);
+            const int y = row0 + (t0 + i) * BN;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(bar, 2 * kKvBytes);
+                tma_load_2d(smem_u32(sK + s * kKvBytes), &tm_kv, (p.heads + kvh) * HD, y, bar);
+            } else if (lane == 1) {
+                tma_load_2d(smem_u32(sV + s * kKvBytes), &tm_kv, (p.heads + p.kv_heads + kvh) * HD,
+                            y, bar);
+            }
+            __syncwarp();
+            ++loaded;
+        }
+        if (lane == 0 && n > 0 && *abort) {
+            // unwinding: every copy in flight lands before the CTA ends
+            mbar_wait(b_q, 0, nullptr, p.status, ST_TIMEOUT_DRAIN, 0);
+            for (int s = 0; s < STAGES && s < loaded; ++s)
+                mbar_wait(smem_u32(&tail->kv_full[s]), ((loaded - s - 1) / STAGES) & 1, nullptr,
+                          p.status, ST_TIMEOUT_DRAIN, s);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------ MMA issuer
+        const bool elected = elect_one();
+        auto wait_all = [&](uint32_t bar, uint32_t parity, uint32_t where) -> bool {
+            bool r = true;
+            if (elected) r = mbar_wait(bar, parity, abort, p.status, ST_TIMEOUT_MMA, where);
+            return __all_sync(kFull, r);
+        };
+        const uint32_t idesc_s = idesc_f16(BM, BN, bf16, bf16, 0, 0);
+        const uint32_t idesc_o = idesc_f16(BM, HD, 0, 0, 0, 1);
+        const uint64_t dq = sdesc_sw128(smem_u32(sQ), 16, 1024);
+        const uint64_t dk = sdesc_sw128(smem_u32(sK), 16, 1024);
+        // V rows are keys with the 64 columns contiguous: the MN-major B
+        // operand, one swizzle atom wide, groups of 8 keys 1024 bytes apart
+        const uint64_t dv = sdesc_sw128(smem_u32(sV), kKvBytes, 1024);
+        constexpr uint64_t kStep = kKvBytes >> 4;
+        const int end = span_of(p, seq).len;
+        bool ok = n == 0 || wait_all(smem_u32(&tail->q_full), 0, 0xFFFF);
+        tc_fence_after();
+        auto issue_s = [&](int i) -> bool {
+            const int st = i % STAGES;
+            if (!wait_all(smem_u32(&tail->kv_full[st]), (i / STAGES) & 1, i)) return false;
+            const int valid = end - (t0 + i) * BN;
+            if (valid < BN) {
+                // the sequence ends inside this tile: its V rows past the
+                // end belong to no key (a whole 128-byte row each, so the
+                // swizzle does not matter)
+                uint8_t* v = sV + st * kKvBytes;
+                for (int r = valid + (lane >> 3); r < BN; r += 4)
+                    *reinterpret_cast<uint4*>(v + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            tc_fence_after();
+            const uint64_t b = dk + st * kStep;
+            const uint32_t dst = tmem + BN * (i % SBUFS);
+            if (elected) {
+                mma_ss(dst, dq, b, idesc_s, 0u);
+#pragma unroll
+                for (int k = 1; k < HD / 16; ++k) mma_ss(dst, dq + 2 * k, b + 2 * k, idesc_s, 1u);
+                mma_commit(smem_u32(&tail->s_full[i % SBUFS]));
+            }
+            __syncwarp();
+            return true;
+        };
+        auto issue_pv = [&](int i) -> bool {
+            if (!wait_all(smem_u32(&tail->p_full[i % SBUFS]), (i / SBUFS) & 1, 0x10000 | i))
+                return false;
+            tc_fence_after();
+            const uint64_t b = dv + (i % STAGES) * kStep;
+            const uint32_t a = tmem + BN * (i % SBUFS);
+            if (elected) {
+                mma_ts(tmem + kColO, a, b, idesc_o, i > 0 ? 1u : 0u);
+#pragma unroll
+                for (int k = 1; k < BN / 16; ++k)
+                    mma_ts(tmem + kColO, a + k * 8, b + 128 * k, idesc_o, 1u);
+                if (i + STAGES < n) mma_commit(smem_u32(&tail->kv_empty[i % STAGES]));
+                mma_commit(smem_u32(&tail->o_done[i & 1]));
+                if (i == n - 1) mma_commit(smem_u32(&tail->o_final));
+            }
+            __syncwarp();
+            return true;
+        };
+        for (int i = 0; i < SBUFS && i < n && ok; ++i) ok = issue_s(i);
+        for (int i = 0; i < n && ok; ++i) {
+            ok = issue_pv(i);
+            if (ok && i + SBUFS < n) ok = issue_s(i + SBUFS);
+        }
+        if (!ok) {
+            // unwinding: what was issued completes before TMEM is released
+            if (elected) {
+                mma_commit(smem_u32(&tail->drain));
+                mbar_wait(smem_u32(&tail->drain), 0, nullptr, p.status, ST_TIMEOUT_DRAIN, 0xD);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------ softmax
+        const int sub = warp & 3;
+        const int row = sub * 32 + lane;
+        const uint32_t t_lane = tmem + (static_cast<uint32_t>(sub * 32) << 16);
+        const uint32_t o_col = t_lane + kColO;
+        const Span q = span_of(p, seq);
+        const int at = tail->q0 + row;  // this row within the sequence
+        const bool live = row < tail->rows;
+        const int seen = live ? visible(p, q, at) : 0;
+        constexpr bool kPlain = !kCap && kBias == BIAS_NONE;
+        // kPlain keeps raw scores and scales them in the exponent's FMA; the
+        // other forms turn each score into log2 units first
+        const float c = kPlain ? p.scale * kLog2e : 1.0f;
+        const float in = kCap ? 2.0f * p.scale / p.cap * kLog2e : p.scale * kLog2e;
+        const float cap2 = p.cap * kLog2e;
+        const float slope2 = kBias != BIAS_NONE ? p.slopes[head] * kLog2e : 0.0f;
+        float qp[3] = {0.0f, 0.0f, 0.0f};
+        if (kBias >= BIAS_PLANE) {
+#pragma unroll
+            for (int a = 0; a < 3; ++a)
+                if (live && a < p.pos_axes) qp[a] = p.pos[(q.begin + at) * p.pos_row + a];
+        }
+        float m_used = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const int k0 = (t0 + i) * BN;
+            if (kBias >= BIAS_PLANE) {
+                __syncwarp();  // every lane is done with the last tile's copy
+                constexpr int kAxes = kBias == BIAS_SPACE ? 3 : 2;
+#pragma unroll
+                for (int a = 0; a < kAxes; ++a)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = k0 + lane + 32 * e;
+                        tail->kpos[sub][a][lane + 32 * e] =
+                            key < q.len && a < p.pos_axes ? p.pos[(q.begin + key) * p.pos_row + a]
+                                                          : 0.0f;
+                    }
+                __syncwarp();
+            }
+            const uint32_t s_col = t_lane + BN * (i % SBUFS);
+            ok = mbar_wait(smem_u32(&tail->s_full[i % SBUFS]), (i / SBUFS) & 1, abort, p.status,
+                           ST_TIMEOUT_SOFTMAX, i);
+            ok = __all_sync(kFull, ok);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[BN];
+            tmem_ld32(s_col, *reinterpret_cast<uint32_t(*)[32]>(s));
+            tmem_ld32(s_col + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+            tmem_wait_ld();
+            if (!kPlain) {
+                const float rel = static_cast<float>(at - k0);
+#pragma unroll
+                for (int k = 0; k < BN; ++k) {
+                    float t = __uint_as_float(s[k]) * in;
+                    if (kCap) t = fmaf(rcp_approx(1.0f + ex2(t)), -2.0f * cap2, cap2);
+                    if (kBias == BIAS_INDEX) t = fmaf(-slope2, fabsf(rel - static_cast<float>(k)), t);
+                    if (kBias >= BIAS_PLANE) {
+                        const float x = qp[0] - tail->kpos[sub][0][k];
+                        const float y = qp[1] - tail->kpos[sub][1][k];
+                        float d2 = fmaf(x, x, y * y);
+                        if (kBias == BIAS_SPACE) {
+                            const float z = qp[2] - tail->kpos[sub][2][k];
+                            d2 = fmaf(z, z, d2);
+                        }
+                        t = fmaf(-slope2, sqrt_approx(d2), t);
+                    }
+                    s[k] = __float_as_uint(t);
+                }
+            }
+            const int valid = seen - k0;
+            if (valid < BN) {
+#pragma unroll
+                for (int k = 0; k < BN; ++k)
+                    if (k >= valid) s[k] = __float_as_uint(-INFINITY);
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int k = 0; k < BN; k += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mx[e] = fmax3(mx[e], __uint_as_float(s[k + 2 * e]),
+                                  __uint_as_float(s[k + 2 * e + 1]));
+            const float m_row = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+            const float m_new = fmaxf(m_used, m_row * c);
+            const bool need = m_new > m_used + kRescaleThreshold;
+            float alpha = 1.0f;
+            if (need) {
+                alpha = ex2(m_used - m_new);
+                l *= alpha;
+                m_used = m_new;
+            }
+            if (i > 0 && __any_sync(kFull, need)) {
+                ok = mbar_wait(smem_u32(&tail->o_done[(i - 1) & 1]), ((i - 1) >> 1) & 1, abort,
+                               p.status, ST_TIMEOUT_SOFTMAX, 0x10000 | i);
+                ok = __all_sync(kFull, ok);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int h = 0; h < HD / 16; ++h) {
+                    uint32_t o[16];
+                    tmem_ld16(o_col + 16 * h, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                    tmem_st16(o_col + 16 * h, o);
+                }
+                tmem_wait_st();
+            }
+            // a row that has seen no key yet (another split's, or none) has no
+            // maximum: its exponents are taken against 0
+            const float nm = m_used == -INFINITY ? 0.0f : -m_used;
+            const unsigned long long nm2 = f2pack(nm, nm), c2 = f2pack(c, c);
+            unsigned long long acc[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = f2pack(0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < BN / 2; ++k) {
+                float x0, x1;
+                f2unpack(ffma2(f2pack(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c2,
+                               nm2), x0, x1);
+                x0 = ex2(x0), x1 = ex2(x1);
+                acc[k & 3] = fadd2(acc[k & 3], f2pack(x0, x1));
+                s[k] = pack_f16x2(x0, x1);
+            }
+            float sa, sb;
+            f2unpack(fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3])), sa, sb);
+            l += sa + sb;
+            tmem_st32(s_col, *reinterpret_cast<uint32_t(*)[32]>(s));
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&tail->p_full[i % SBUFS]));
+        }
+        if (ok && n > 0)
+            ok = mbar_wait(smem_u32(&tail->o_final), 0, abort, p.status, ST_TIMEOUT_SOFTMAX, 0x20000);
+        ok = __all_sync(kFull, ok);
+        float o[HD];
+        if (ok && n > 0) {
+            tc_fence_after();
+            tmem_ld32(o_col, *reinterpret_cast<uint32_t(*)[32]>(o));
+            tmem_ld32(o_col + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+            tmem_wait_ld();
+        }
+        if (p.splits == 1) {
+            if (ok && live) {
+                const float inv = 1.0f / l;
+                const long long to = (q.begin + at) * p.out_row + head * HD;
+#pragma unroll
+                for (int k = 0; k < HD; k += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = o[k + e] * inv;
+                    store8(p.out, to + k, p.out_dtype, v);
+                }
+            }
+        } else {
+            // the split's O, (max, sum) of each row into the K ring, free by
+            // now (the last PV is complete, so every copy has landed and been
+            // read); vectors of a row rotated so that a warp's stores spread
+            // over the banks
+            float4* po = reinterpret_cast<float4*>(sK);
+            const bool some = ok && n > 0;
+#pragma unroll
+            for (int k = 0; k < HD / 4; ++k)
+                po[row * 16 + (k ^ (row & 15))] =
+                    some ? make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3])
+                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            reinterpret_cast<float2*>(sV)[row] = make_float2(some ? m_used : -INFINITY,
+                                                             some ? l : 0.0f);
+        }
+    }
+    if (p.splits > 1) {
+        // The cluster's CTAs share out the tile's rows; each adds every
+        // split's part of its rows in rank order (the same bits in every run).
+        __syncwarp();
+        fence_cluster();
+        cluster_sync();
+        const int me = static_cast<int>(cluster_rank());
+        const int r0 = BM * me / p.splits, r1 = min(BM * (me + 1) / p.splits, tail->rows);
+        const Span q = span_of(p, seq);
+        for (int i = r0 * 16 + threadIdx.x; i < r1 * 16; i += kTileThreads) {
+            const int row = i >> 4, k = i & 15;
+            float top = -INFINITY;
+            for (int s = 0; s < p.splits; ++s)
+                top = fmaxf(top, dsmem_ld2(dsmem_addr(smem_u32(sV) + row * 8, s)).x);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float sum = 0.0f;
+            for (int s = 0; s < p.splits; ++s) {
+                const float2 ml = dsmem_ld2(dsmem_addr(smem_u32(sV) + row * 8, s));
+                const float w = ex2(ml.x - ref);
+                const float4 v = dsmem_ld4(
+                    dsmem_addr(smem_u32(sK) + (row * 16 + (k ^ (row & 15))) * 16, s));
+                sum = fmaf(w, ml.y, sum);
+                a.x = fmaf(w, v.x, a.x), a.y = fmaf(w, v.y, a.y);
+                a.z = fmaf(w, v.z, a.z), a.w = fmaf(w, v.w, a.w);
+            }
+            const float inv = 1.0f / sum;
+            store4(p.out, (q.begin + tail->q0 + row) * p.out_row + head * HD + 4 * k, p.out_dtype,
+                   make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+        }
+        cluster_sync();  // no CTA leaves while its part is read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
 int validate(const bl_masked_attention_args& a) {
     if (a.head_dim != HD)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: head_dim %u (only 64)", a.head_dim);
@@ -295,7 +839,7 @@ int validate(const bl_masked_attention_args& a) {
     if (a.offsets != nullptr && a.lengths != nullptr)
         return fail(BL_ERR_INVALID, "masked attention: offsets (packed) and lengths (padded)");
     const uint64_t rows = a.offsets != nullptr ? a.tokens : 1ull * a.batch * a.tokens;
-    if (a.tokens > 0x7FFFFFFFu || a.batch > 0x7FFFFFFEu || rows > 0x7FFFFFFFull)
+    if (a.tokens > 0x7FFFFFFFu || a.batch > 0x7FFF0000u || rows > 0x7FFFFFFFull)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: %u sequences of %u rows", a.batch, a.tokens);
     if (a.qk_dtype != BL_F16 && a.qk_dtype != BL_BF16)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: Q/K dtype %d (f16 or bf16)", a.qk_dtype);
@@ -385,11 +929,69 @@ int prepare_rows(const bl_masked_attention_args& a, Launch* out) {
     return BL_OK;
 }
 
+int prepare_tiles(const bl_masked_attention_args& a, Launch* out) {
+    Params p = params_of(a);
+    // Tiles: a packed batch has at most one short tile a sequence beside its
+    // whole ones; the kernel finds which exist (chunks = 0). Otherwise every
+    // sequence has as many as its longest form.
+    const bool packed = a.offsets != nullptr && p.last_rows == 0;
+    const uint64_t per_seq = ((p.last_rows > 0 ? p.last_rows : p.tokens) + BM - 1ull) / BM;
+    const uint64_t units = packed ? p.tokens / BM + std::min<uint64_t>(a.batch, a.tokens)
+                                  : per_seq * a.batch;
+    p.chunks = packed ? 0 : static_cast<int>(per_seq);
+    // Split the keys while that many CTAs still run at once (two an SM) and
+    // each keeps 256 keys of an average sequence.
+    const uint64_t keys = a.offsets != nullptr ? a.tokens / a.batch : a.tokens;
+    p.splits = a.key_splits ? static_cast<int>(a.key_splits)
+                            : static_cast<int>(std::max<uint64_t>(
+                                  1, std::min<uint64_t>({8, 296 / (units * p.heads), keys / 256})));
+    if (units * p.splits > 0x7FFFFFFFull)
+        return fail(BL_ERR_UNSUPPORTED, "masked attention: grid too large");
+    const uint64_t rows = a.offsets != nullptr ? a.tokens : 1ull * a.batch * a.tokens;
+    CUtensorMap tm_q, tm_kv;
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.heads + 2 * p.kv_heads) * HD, rows};
+    const uint32_t qbox[2] = {HD, BM}, kbox[2] = {HD, BN};
+    int rc = make_tmap_16bit_2d(&tm_q, a.qkv, dims, static_cast<uint64_t>(p.row) * 2, qbox);
+    if (rc == BL_OK)
+        rc = make_tmap_16bit_2d(&tm_kv, a.qkv, dims, static_cast<uint64_t>(p.row) * 2, kbox);
+    if (rc != BL_OK) return rc;
+    using Kern = void (*)(const CUtensorMap, const CUtensorMap, const Params, int);
+    static const Kern kerns[2][4] = {
+        {tile_kernel<false, BIAS_NONE>, tile_kernel<false, BIAS_INDEX>,
+         tile_kernel<false, BIAS_PLANE>, tile_kernel<false, BIAS_SPACE>},
+        {tile_kernel<true, BIAS_NONE>, tile_kernel<true, BIAS_INDEX>,
+         tile_kernel<true, BIAS_PLANE>, tile_kernel<true, BIAS_SPACE>}};
+    const int bias = p.slopes == nullptr ? BIAS_NONE
+                     : p.pos == nullptr  ? BIAS_INDEX
+                     : p.pos_axes <= 2   ? BIAS_PLANE
+                                         : BIAS_SPACE;
+    const Kern kern = kerns[p.cap > 0.0f ? 1 : 0][bias];
+    BL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(kTileSmem)));
+    const dim3 grid(static_cast<unsigned>(units * p.splits), p.heads);
+    const int bf16 = a.qk_dtype == BL_BF16;
+    out->op = BL_OP_MASKED_ATTENTION;
+    out->run = [=](cudaStream_t s) {
+        return p.splits > 1 ? launch_k_cluster(kern, grid, dim3(kTileThreads), dim3(p.splits, 1, 1),
+                                               kTileSmem, s, tm_q, tm_kv, p, bf16)
+                            : launch_k(kern, grid, dim3(kTileThreads), kTileSmem, s, tm_q, tm_kv, p,
+                                       bf16);
+    };
+    return BL_OK;
+}
+
 }  // namespace masked
 
 int prepare_masked_attention(const bl_masked_attention_args& a, Launch* out) {
     const int rc = masked::validate(a);
-    return rc != BL_OK ? rc : masked::prepare_rows(a, out);
+    if (rc != BL_OK) return rc;
+    // The last rows of a stream: while a K/V head's query rows are few, the
+    // tensor cores' 128-row tile would be nearly empty and the keys' bytes
+    // are what counts.
+    const uint32_t kv = a.kv_heads ? a.kv_heads : a.heads;
+    const uint64_t combos = 1ull * std::min(a.last_rows, a.tokens) * (a.heads / kv);
+    return a.last_rows > 0 && combos <= 4 ? masked::prepare_rows(a, out)
+                                          : masked::prepare_tiles(a, out);
 }
 
 }  // namespace bl
