@@ -285,25 +285,37 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(const Params p, int b
 // ------------------------------------------------------------------ tiles
 //
 // One CTA computes 128 query rows of one head over a range of 64-key tiles on
-// the tensor cores; two CTAs share an SM (256 threads of at most 128
-// registers, half the TMEM each), so one's exponentials run beside the
-// other's waits and a tile's set-up and end are hidden by its neighbour.
+// the tensor cores; two CTAs share an SM, with half the TMEM each. The
+// exponentials bound it (one a score at 16 a clock and SM, against a quarter
+// of that time for its products), so the rest is there to keep that unit fed.
+// Every query row has two softmax threads, one for the even key tiles and one
+// for the odd, so four softmax warps a scheduler cover one another's waits;
+// S has three TMEM buffers, so the scores of the next tile are there before a
+// thread asks for them. Both add to one O, whose reference exponent R (the
+// lagging running maximum) they hand to each other: R(i) follows from R(i - 1)
+// and the maximum of tile i, known long before tile i's exponentials are done.
 // Warps:
-//   0     TMA producer: the Q tile once, then K and V tiles into a ring.
-//   1     MMA issuer: S = Q K^T (M 128, N 64, K 64) into one of three TMEM
-//         buffers, O += P V (P from TMEM, f16). S of tile i + 3 follows
-//         PV(i) in the tensor pipe, whose buffer it takes.
-//   2     finds the CTA's sequence among the packed ones.
-//   4..7  softmax, one thread a query row (TMEM lane).
+//   0      finds the CTA's sequence among the packed ones, then the TMA
+//          producer: the Q tile once, then K and V tiles into a ring.
+//   1      MMA issuer: S = Q K^T (M 128, N 64, K 64) into TMEM, O += P V (P
+//          from TMEM, f16, over the S it came from); S(i + 3) follows PV(i),
+//          whose buffer it takes.
+//   2..5   softmax of the even key tiles, one thread a query row (TMEM lane),
+//   6..9   of the odd ones.
+// A thread reads its 64 scores from TMEM twice, 32 at a time, for the maximum
+// and for the exponentials (a 32-column load takes 17 clocks of a warp
+// scheduler's TMEM port, 32 exponentials 256), which leaves it within the 96
+// registers that ten warps and two CTAs allow.
 // Tiles start at their sequence's first row, so a key tile holds keys of one
 // sequence, and past its end only rows that no query sees: their scores are
 // replaced by -inf and their V rows zeroed in shared memory before the
 // product, since 0 * NaN from another sequence's rows would reach O.
 constexpr int BM = 128;
 constexpr int BN = 64;
-constexpr int STAGES = 5;
+constexpr int STAGES = 5;  // K/V ring
 constexpr int SBUFS = 3;
-constexpr int kTileThreads = 256;
+constexpr int kTileThreads = 320;  // two CTAs of 96 registers a thread
+constexpr int kSoftmaxWarp0 = 2;
 constexpr uint32_t kQBytes = BM * HD * 2;
 constexpr uint32_t kKvBytes = BN * HD * 2;
 constexpr uint32_t kTmemCols = 256;
@@ -317,12 +329,14 @@ struct TileTail {
     uint64_t q_full;
     uint64_t kv_full[STAGES];
     uint64_t kv_empty[STAGES];
-    uint64_t s_full[SBUFS];  // by S buffer: at most one phase ahead, as S(i + 3) waits for P(i)
+    // by S buffer (tile i: i % SBUFS). S(i) complete means that S(i - 1) and
+    // PV(i - 3) are, so each parity names one phase wherever it is waited for.
+    uint64_t s_full[SBUFS];
     uint64_t p_full[SBUFS];
-    // by parity of the key tile: when the softmax of tile i asks for PV(i - 1),
-    // PV(i - 3) is done (S(i) followed it), so the parity names one phase
-    uint64_t o_done[2];
+    uint64_t o_done[SBUFS];  // PV(i) is complete
+    uint64_t ref_full[2][4]; // R of the stream's tile is written, by TMEM quarter
     uint64_t o_final;
+    uint64_t odd_done;       // the odd stream's sums are written
     uint64_t drain;
     uint32_t tmem_base;
     int abort;
@@ -331,7 +345,9 @@ struct TileTail {
     int q0, rows;   // first query row within the sequence, rows of the tile
     int keys;       // keys that some row of the tile sees
     int t0, n;      // its key tiles
-    float kpos[4][3][BN];  // each softmax warp's copy of a key tile's positions
+    float ref[2][BM];      // R after the stream's last tile
+    float odd_sum[BM];
+    float kpos[8][3][BN];  // each softmax warp's copy of a key tile's positions
 };
 constexpr size_t kTileSmem = 1024 + kQBytes + 2 * STAGES * kKvBytes + sizeof(TileTail);
 static_assert(2 * (kTileSmem + 1024) <= 233472, "two CTAs an SM");
@@ -424,7 +440,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* sQ = smem;
-    uint8_t* sK = smem + kQBytes;                       // stage s at + s * kKvBytes
+    uint8_t* sK = smem + kQBytes;  // stage s at + s * kKvBytes
     uint8_t* sV = sK + STAGES * kKvBytes;
     TileTail* tail = reinterpret_cast<TileTail*>(sV + STAGES * kKvBytes);
     volatile int* abort = &tail->abort;
@@ -434,17 +450,18 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&tail->q_full), 1);
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(smem_u32(&tail->kv_full[s]), 1);
-            mbar_init(smem_u32(&tail->kv_empty[s]), 1);
+        for (int t = 0; t < STAGES; ++t) {
+            mbar_init(smem_u32(&tail->kv_full[t]), 1);
+            mbar_init(smem_u32(&tail->kv_empty[t]), 1);
         }
-        for (int s = 0; s < SBUFS; ++s) {
-            mbar_init(smem_u32(&tail->s_full[s]), 1);
-            mbar_init(smem_u32(&tail->p_full[s]), BM);
+        for (int t = 0; t < SBUFS; ++t) {
+            mbar_init(smem_u32(&tail->s_full[t]), 1);
+            mbar_init(smem_u32(&tail->p_full[t]), 4);  // one arrival a warp
+            mbar_init(smem_u32(&tail->o_done[t]), 1);
         }
-        mbar_init(smem_u32(&tail->o_done[0]), 1);
-        mbar_init(smem_u32(&tail->o_done[1]), 1);
+        for (int t = 0; t < 8; ++t) mbar_init(smem_u32(&tail->ref_full[t >> 2][t & 3]), 1);
         mbar_init(smem_u32(&tail->o_final), 1);
+        mbar_init(smem_u32(&tail->odd_done), 4);
         mbar_init(smem_u32(&tail->drain), 1);
         tail->abort = 0;
         fence_barrier_init();
@@ -458,7 +475,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     }
     pdl_trigger();
     pdl_wait();
-    if (warp == 2) {
+    if (warp == 0) {
+        __syncwarp();
         const int unit = static_cast<int>(blockIdx.x) / p.splits;
         const int split = static_cast<int>(blockIdx.x) % p.splits;
         int seq, tile;
@@ -500,38 +518,40 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     }
     const int t0 = tail->t0, n = tail->n;
 
+    // One lane waits and the vote hands its outcome to the warp, unless the
+    // barrier is past that phase already.
+    const bool elected = elect_one();
+    auto wait_warp = [&](uint64_t* bar, int parity, uint32_t code, uint32_t where) -> bool {
+        if (__all_sync(kFull, mbar_try_wait(smem_u32(bar), parity))) return true;
+        bool r = true;
+        if (elected) r = mbar_wait(smem_u32(bar), parity, abort, p.status, code, where);
+        return __all_sync(kFull, r);
+    };
     if (warp == 0) {
         // ------------------------------------------------------ producer
-        const Span q = span_of(p, seq);
-        const int row0 = static_cast<int>(q.begin);
-        const uint32_t b_q = smem_u32(&tail->q_full);
-        if (lane == 0 && n > 0) {
-            mbar_arrive_expect_tx(b_q, kQBytes);
-            tma_load_2d(smem_u32(sQ), &tm_q, head * HD, row0 + tail->q0, b_q);
+        const int row0 = static_cast<int>(span_of(p, seq).begin);
+        if (elected && n > 0) {
+            mbar_arrive_expect_tx(smem_u32(&tail->q_full), kQBytes);
+            tma_load_2d(smem_u32(sQ), &tm_q, head * HD, row0 + tail->q0, smem_u32(&tail->q_full));
         }
         int loaded = 0;
-        for (int i = 0; i < n; ++i) {
-            const int s = i % STAGES, r = i / STAGES;
-            bool w = true;
-            if (lane == 0 && r > 0)
-                w = mbar_wait(smem_u32(&tail->kv_empty[s]), (r - 1) & 1, abort, p.status,
-                              ST_TIMEOUT_TMA, i);
-            if (!__all_sync(kFull, w)) break;
+        for (int i = 0, s = 0, phase = 1; i < n; ++i) {
+            if (i >= STAGES && !wait_warp(&tail->kv_empty[s], phase, ST_TIMEOUT_TMA, i)) break;
             const uint32_t bar = smem_u32(&tail->kv_full[s]);
             const int y = row0 + (t0 + i) * BN;
-            if (lane == 0) {
+            if (elected) {
                 mbar_arrive_expect_tx(bar, 2 * kKvBytes);
                 tma_load_2d(smem_u32(sK + s * kKvBytes), &tm_kv, (p.heads + kvh) * HD, y, bar);
-            } else if (lane == 1) {
                 tma_load_2d(smem_u32(sV + s * kKvBytes), &tm_kv, (p.heads + p.kv_heads + kvh) * HD,
                             y, bar);
             }
             __syncwarp();
             ++loaded;
+            if (++s == STAGES) s = 0, phase ^= 1;
         }
-        if (lane == 0 && n > 0 && *abort) {
+        if (elected && n > 0 && *abort) {
             // unwinding: every copy in flight lands before the CTA ends
-            mbar_wait(b_q, 0, nullptr, p.status, ST_TIMEOUT_DRAIN, 0);
+            mbar_wait(smem_u32(&tail->q_full), 0, nullptr, p.status, ST_TIMEOUT_DRAIN, 0);
             for (int s = 0; s < STAGES && s < loaded; ++s)
                 mbar_wait(smem_u32(&tail->kv_full[s]), ((loaded - s - 1) / STAGES) & 1, nullptr,
                           p.status, ST_TIMEOUT_DRAIN, s);
@@ -539,12 +559,6 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------ MMA issuer
-        const bool elected = elect_one();
-        auto wait_all = [&](uint32_t bar, uint32_t parity, uint32_t where) -> bool {
-            bool r = true;
-            if (elected) r = mbar_wait(bar, parity, abort, p.status, ST_TIMEOUT_MMA, where);
-            return __all_sync(kFull, r);
-        };
         const uint32_t idesc_s = idesc_f16(BM, BN, bf16, bf16, 0, 0);
         const uint32_t idesc_o = idesc_f16(BM, HD, 0, 0, 0, 1);
         const uint64_t dq = sdesc_sw128(smem_u32(sQ), 16, 1024);
@@ -554,11 +568,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         const uint64_t dv = sdesc_sw128(smem_u32(sV), kKvBytes, 1024);
         constexpr uint64_t kStep = kKvBytes >> 4;
         const int end = span_of(p, seq).len;
-        bool ok = n == 0 || wait_all(smem_u32(&tail->q_full), 0, 0xFFFF);
-        tc_fence_after();
-        auto issue_s = [&](int i) -> bool {
-            const int st = i % STAGES;
-            if (!wait_all(smem_u32(&tail->kv_full[st]), (i / STAGES) & 1, i)) return false;
+        // ring places, stepped as the loop goes: S runs SBUFS tiles ahead of PV
+        int sb = 0, st = 0, st_phase = 0;  // of the next S: TMEM buffer, stage
+        int pb = 0, p_phase = 0, pt = 0;   // of the next PV
+        auto wait_tile = [&](int i) -> bool {
+            if (!wait_warp(&tail->kv_full[st], st_phase, ST_TIMEOUT_MMA, i)) return false;
             const int valid = end - (t0 + i) * BN;
             if (valid < BN) {
                 // the sequence ends inside this tile: its V rows past the
@@ -570,40 +584,51 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 fence_proxy_async_smem();
                 __syncwarp();
             }
-            tc_fence_after();
+            return true;
+        };
+        auto issue_s = [&]() {
             const uint64_t b = dk + st * kStep;
-            const uint32_t dst = tmem + BN * (i % SBUFS);
+            const uint32_t dst = tmem + BN * sb;
             if (elected) {
                 mma_ss(dst, dq, b, idesc_s, 0u);
 #pragma unroll
                 for (int k = 1; k < HD / 16; ++k) mma_ss(dst, dq + 2 * k, b + 2 * k, idesc_s, 1u);
-                mma_commit(smem_u32(&tail->s_full[i % SBUFS]));
+                mma_commit(smem_u32(&tail->s_full[sb]));
             }
             __syncwarp();
-            return true;
+            if (++sb == SBUFS) sb = 0;
+            if (++st == STAGES) st = 0, st_phase ^= 1;
         };
-        auto issue_pv = [&](int i) -> bool {
-            if (!wait_all(smem_u32(&tail->p_full[i % SBUFS]), (i / SBUFS) & 1, 0x10000 | i))
-                return false;
-            tc_fence_after();
-            const uint64_t b = dv + (i % STAGES) * kStep;
-            const uint32_t a = tmem + BN * (i % SBUFS);
+        auto issue_pv = [&](int i) {
+            const uint64_t b = dv + pt * kStep;
+            const uint32_t a = tmem + BN * pb, o = tmem + kColO;
             if (elected) {
-                mma_ts(tmem + kColO, a, b, idesc_o, i > 0 ? 1u : 0u);
+                mma_ts(o, a, b, idesc_o, i > 0 ? 1u : 0u);
 #pragma unroll
-                for (int k = 1; k < BN / 16; ++k)
-                    mma_ts(tmem + kColO, a + k * 8, b + 128 * k, idesc_o, 1u);
-                if (i + STAGES < n) mma_commit(smem_u32(&tail->kv_empty[i % STAGES]));
-                mma_commit(smem_u32(&tail->o_done[i & 1]));
+                for (int k = 1; k < BN / 16; ++k) mma_ts(o, a + k * 8, b + 128 * k, idesc_o, 1u);
+                mma_commit(smem_u32(&tail->o_done[pb]));
+                if (i + STAGES < n) mma_commit(smem_u32(&tail->kv_empty[pt]));
                 if (i == n - 1) mma_commit(smem_u32(&tail->o_final));
             }
             __syncwarp();
-            return true;
+            if (++pb == SBUFS) pb = 0, p_phase ^= 1;
+            if (++pt == STAGES) pt = 0;
         };
-        for (int i = 0; i < SBUFS && i < n && ok; ++i) ok = issue_s(i);
+        bool ok = n == 0 || wait_warp(&tail->q_full, 0, ST_TIMEOUT_MMA, 0xFFFF);
+        for (int i = 0; i < SBUFS && i < n && ok; ++i) {
+            ok = wait_tile(i);
+            tc_fence_after();
+            if (ok) issue_s();
+        }
         for (int i = 0; i < n && ok; ++i) {
-            ok = issue_pv(i);
-            if (ok && i + SBUFS < n) ok = issue_s(i + SBUFS);
+            // what S(i + 3) needs first: between P(i) and it stand only MMAs
+            const bool more = i + SBUFS < n;
+            if (more) ok = wait_tile(i + SBUFS);
+            ok = ok && wait_warp(&tail->p_full[pb], p_phase, ST_TIMEOUT_MMA, 0x10000 | i);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(i);
+            if (more) issue_s();
         }
         if (!ok) {
             // unwinding: what was issued completes before TMEM is released
@@ -613,9 +638,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             }
             __syncwarp();
         }
-    } else if (warp >= 4) {
+    } else {
         // ------------------------------------------------------ softmax
         const int sub = warp & 3;
+        const int odd = (warp - kSoftmaxWarp0) >> 2;  // the stream
         const int row = sub * 32 + lane;
         const uint32_t t_lane = tmem + (static_cast<uint32_t>(sub * 32) << 16);
         const uint32_t o_col = t_lane + kColO;
@@ -636,9 +662,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             for (int a = 0; a < 3; ++a)
                 if (live && a < p.pos_axes) qp[a] = p.pos[(q.begin + at) * p.pos_row + a];
         }
-        float m_used = -INFINITY, l = 0.0f;
+        const float(*kpos)[BN] = tail->kpos[warp - kSoftmaxWarp0];
+        float m_used = -INFINITY, l = 0.0f;  // R as this thread last knew it; l is relative to it
         bool ok = true;
-        for (int i = 0; i < n; ++i) {
+        // tile i: S buffer `buf` = i % SBUFS, whose use it is the phase of
+        int buf = odd, phase = 0;
+        for (int i = odd; i < n; i += 2) {
             const int k0 = (t0 + i) * BN;
             if (kBias >= BIAS_PLANE) {
                 __syncwarp();  // every lane is done with the last tile's copy
@@ -648,70 +677,83 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int key = k0 + lane + 32 * e;
-                        tail->kpos[sub][a][lane + 32 * e] =
+                        tail->kpos[warp - kSoftmaxWarp0][a][lane + 32 * e] =
                             key < q.len && a < p.pos_axes ? p.pos[(q.begin + key) * p.pos_row + a]
                                                           : 0.0f;
                     }
                 __syncwarp();
             }
-            const uint32_t s_col = t_lane + BN * (i % SBUFS);
-            ok = mbar_wait(smem_u32(&tail->s_full[i % SBUFS]), (i / SBUFS) & 1, abort, p.status,
-                           ST_TIMEOUT_SOFTMAX, i);
-            ok = __all_sync(kFull, ok);
+            const uint32_t s_col = t_lane + BN * buf;
+            ok = wait_warp(&tail->s_full[buf], phase, ST_TIMEOUT_SOFTMAX, i);
             if (!ok) break;
             tc_fence_after();
-            uint32_t s[BN];
-            tmem_ld32(s_col, *reinterpret_cast<uint32_t(*)[32]>(s));
-            tmem_ld32(s_col + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
-            tmem_wait_ld();
-            if (!kPlain) {
-                const float rel = static_cast<float>(at - k0);
-#pragma unroll
-                for (int k = 0; k < BN; ++k) {
-                    float t = __uint_as_float(s[k]) * in;
-                    if (kCap) t = fmaf(rcp_approx(1.0f + ex2(t)), -2.0f * cap2, cap2);
-                    if (kBias == BIAS_INDEX) t = fmaf(-slope2, fabsf(rel - static_cast<float>(k)), t);
-                    if (kBias >= BIAS_PLANE) {
-                        const float x = qp[0] - tail->kpos[sub][0][k];
-                        const float y = qp[1] - tail->kpos[sub][1][k];
-                        float d2 = fmaf(x, x, y * y);
-                        if (kBias == BIAS_SPACE) {
-                            const float z = qp[2] - tail->kpos[sub][2][k];
-                            d2 = fmaf(z, z, d2);
-                        }
-                        t = fmaf(-slope2, sqrt_approx(d2), t);
-                    }
-                    s[k] = __float_as_uint(t);
-                }
-            }
             const int valid = seen - k0;
-            if (valid < BN) {
-#pragma unroll
-                for (int k = 0; k < BN; ++k)
-                    if (k >= valid) s[k] = __float_as_uint(-INFINITY);
-            }
+            const float rel = static_cast<float>(at - k0);
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int k = 0; k < BN; k += 8)
+            for (int h = 0; h < 2; ++h) {
+                uint32_t s[32];
+                tmem_ld32(s_col + 32 * h, s);
+                tmem_wait_ld();
+                if (!kPlain) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    mx[e] = fmax3(mx[e], __uint_as_float(s[k + 2 * e]),
-                                  __uint_as_float(s[k + 2 * e + 1]));
-            const float m_row = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
-            const float m_new = fmaxf(m_used, m_row * c);
-            const bool need = m_new > m_used + kRescaleThreshold;
-            float alpha = 1.0f;
-            if (need) {
-                alpha = ex2(m_used - m_new);
-                l *= alpha;
-                m_used = m_new;
+                    for (int e = 0; e < 32; ++e) {
+                        const int k = 32 * h + e;
+                        float t = __uint_as_float(s[e]) * in;
+                        if (kCap) t = fmaf(rcp_approx(1.0f + ex2(t)), -2.0f * cap2, cap2);
+                        if (kBias == BIAS_INDEX)
+                            t = fmaf(-slope2, fabsf(rel - static_cast<float>(k)), t);
+                        if (kBias >= BIAS_PLANE) {
+                            const float x = qp[0] - kpos[0][k], y = qp[1] - kpos[1][k];
+                            float d2 = fmaf(x, x, y * y);
+                            if (kBias == BIAS_SPACE) {
+                                const float z = qp[2] - kpos[2][k];
+                                d2 = fmaf(z, z, d2);
+                            }
+                            t = fmaf(-slope2, sqrt_approx(d2), t);
+                        }
+                        s[e] = __float_as_uint(t);
+                    }
+                }
+                if (valid < 32 * h + 32) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (32 * h + e >= valid) s[e] = __float_as_uint(-INFINITY);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mx[j] = fmax3(mx[j], __uint_as_float(s[e + 2 * j]),
+                                      __uint_as_float(s[e + 2 * j + 1]));
+                if (!kPlain) tmem_st32(s_col + 32 * h, s);
             }
-            if (i > 0 && __any_sync(kFull, need)) {
-                ok = mbar_wait(smem_u32(&tail->o_done[(i - 1) & 1]), ((i - 1) >> 1) & 1, abort,
-                               p.status, ST_TIMEOUT_SOFTMAX, 0x10000 | i);
-                ok = __all_sync(kFull, ok);
+            if (!kPlain) tmem_wait_st();
+            const float m_row = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+            // R(i) from R(i - 1), the other stream's, and this tile's maximum
+            float prev = -INFINITY;
+            if (i > 0) {
+                ok = wait_warp(&tail->ref_full[odd ^ 1][sub], ((i - 1) >> 1) & 1, ST_TIMEOUT_SOFTMAX,
+                               0x10000 | i);
+                if (!ok) break;
+                prev = tail->ref[odd ^ 1][row];
+            }
+            const float m_new = fmaxf(prev, m_row * c);
+            const bool need = m_new > prev + kRescaleThreshold;
+            const float now = need ? m_new : prev;
+            tail->ref[odd][row] = now;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tail->ref_full[odd][sub]));
+            // raised here or by the other stream: rare after the first tiles
+            const bool raised = __any_sync(kFull, now != m_used);
+            if (raised) l *= now != m_used ? ex2(m_used - now) : 1.0f;
+            m_used = now;
+            if (raised && i > 0 && __any_sync(kFull, need)) {
+                ok = wait_warp(&tail->o_done[(i - 1) % SBUFS], ((i - 1) / SBUFS) & 1,
+                               ST_TIMEOUT_SOFTMAX, 0x20000 | i);
                 if (!ok) break;
                 tc_fence_after();
+                const float alpha = need ? ex2(prev - now) : 1.0f;
 #pragma unroll
                 for (int h = 0; h < HD / 16; ++h) {
                     uint32_t o[16];
@@ -728,62 +770,83 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             // maximum: its exponents are taken against 0
             const float nm = m_used == -INFINITY ? 0.0f : -m_used;
             const unsigned long long nm2 = f2pack(nm, nm), c2 = f2pack(c, c);
-            unsigned long long acc[4];
+            unsigned long long acc[2] = {f2pack(0.0f, 0.0f), f2pack(0.0f, 0.0f)};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = f2pack(0.0f, 0.0f);
+            for (int h = 0; h < 2; ++h) {
+                uint32_t s[32];
+                tmem_ld32(s_col + 32 * h, s);
+                tmem_wait_ld();
+                if (kPlain && valid < 32 * h + 32) {
 #pragma unroll
-            for (int k = 0; k < BN / 2; ++k) {
-                float x0, x1;
-                f2unpack(ffma2(f2pack(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c2,
-                               nm2), x0, x1);
-                x0 = ex2(x0), x1 = ex2(x1);
-                acc[k & 3] = fadd2(acc[k & 3], f2pack(x0, x1));
-                s[k] = pack_f16x2(x0, x1);
+                    for (int e = 0; e < 32; ++e)
+                        if (32 * h + e >= valid) s[e] = __float_as_uint(-INFINITY);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float x0, x1;
+                    f2unpack(ffma2(f2pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])),
+                                   c2, nm2), x0, x1);
+                    x0 = ex2(x0), x1 = ex2(x1);
+                    acc[e & 1] = fadd2(acc[e & 1], f2pack(x0, x1));
+                    s[e] = pack_f16x2(x0, x1);
+                }
+                // P's columns [16 h, 16 h + 16) lie over scores already read
+                tmem_st16(s_col + 16 * h, s);
             }
             float sa, sb;
-            f2unpack(fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3])), sa, sb);
+            f2unpack(fadd2(acc[0], acc[1]), sa, sb);
             l += sa + sb;
-            tmem_st32(s_col, *reinterpret_cast<uint32_t(*)[32]>(s));
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(smem_u32(&tail->p_full[i % SBUFS]));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[buf]));
+            buf += 2;
+            if (buf >= SBUFS) buf -= SBUFS, phase ^= 1;
         }
-        if (ok && n > 0)
-            ok = mbar_wait(smem_u32(&tail->o_final), 0, abort, p.status, ST_TIMEOUT_SOFTMAX, 0x20000);
-        ok = __all_sync(kFull, ok);
-        float o[HD];
-        if (ok && n > 0) {
+        if (odd) {
+            tail->odd_sum[row] = l;
+            tail->ref[1][row] = m_used;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tail->odd_done));
+        } else {
+            ok = ok && wait_warp(&tail->odd_done, 0, ST_TIMEOUT_SOFTMAX, 0x30000);
+            if (ok && n > 0) ok = wait_warp(&tail->o_final, 0, ST_TIMEOUT_SOFTMAX, 0x40000);
             tc_fence_after();
-            tmem_ld32(o_col, *reinterpret_cast<uint32_t(*)[32]>(o));
-            tmem_ld32(o_col + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
-            tmem_wait_ld();
-        }
-        if (p.splits == 1) {
-            if (ok && live) {
-                const float inv = 1.0f / l;
-                const long long to = (q.begin + at) * p.out_row + head * HD;
+            // O is relative to the last R, the larger of the two
+            const float other = ok ? tail->ref[1][row] : -INFINITY;
+            const float top = ok ? fmaxf(m_used, other) : -INFINITY;
+            const float ref = top == -INFINITY ? 0.0f : top;
+            const float sum = ok ? ex2(m_used - ref) * l + ex2(other - ref) * tail->odd_sum[row] : 0.0f;
+            const float w = p.splits == 1 ? 1.0f / sum : 1.0f;
+            const long long to = (q.begin + at) * p.out_row + head * HD;
+            float4* po = reinterpret_cast<float4*>(sK);
 #pragma unroll
-                for (int k = 0; k < HD; k += 8) {
-                    float v[8];
+            for (int h = 0; h < HD / 16; ++h) {
+                uint32_t a[16];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = o[k + e] * inv;
-                    store8(p.out, to + k, p.out_dtype, v);
+                for (int k = 0; k < 16; ++k) a[k] = 0;
+                if (ok && n > 0) tmem_ld16(o_col + 16 * h, a);
+                tmem_wait_ld();
+                float v[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = w * __uint_as_float(a[k]);
+                if (p.splits == 1) {
+                    if (ok && live) {
+                        store8(p.out, to + 16 * h, p.out_dtype, v);
+                        store8(p.out, to + 16 * h + 8, p.out_dtype, v + 8);
+                    }
+                } else {
+                    // the split's O of each row into the K ring, free by now
+                    // (the last PV is complete, so every copy has landed and
+                    // been read); a row's vectors rotated so that a warp's
+                    // stores spread over the banks
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        po[row * 16 + ((4 * h + k) ^ (row & 15))] =
+                            make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
                 }
             }
-        } else {
-            // the split's O, (max, sum) of each row into the K ring, free by
-            // now (the last PV is complete, so every copy has landed and been
-            // read); vectors of a row rotated so that a warp's stores spread
-            // over the banks
-            float4* po = reinterpret_cast<float4*>(sK);
-            const bool some = ok && n > 0;
-#pragma unroll
-            for (int k = 0; k < HD / 4; ++k)
-                po[row * 16 + (k ^ (row & 15))] =
-                    some ? make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3])
-                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            reinterpret_cast<float2*>(sV)[row] = make_float2(some ? m_used : -INFINITY,
-                                                             some ? l : 0.0f);
+            if (p.splits > 1) reinterpret_cast<float2*>(sV)[row] = make_float2(top, sum);
         }
     }
     if (p.splits > 1) {
