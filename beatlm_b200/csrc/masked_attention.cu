@@ -279,7 +279,10 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(const Params p, int b
             else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o);
         }
     }
-    if (p.splits > 1) cluster_sync();  // no CTA leaves while its partials are read
+    if (p.splits > 1) {
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while its partials are read
+    }
 }
 
 // ------------------------------------------------------------------ tiles
@@ -340,10 +343,9 @@ struct TileTail {
     uint64_t drain;
     uint32_t tmem_base;
     int abort;
-    // this CTA's work, found once
-    int seq;        // -1: none
-    int q0, rows;   // first query row within the sequence, rows of the tile
-    int keys;       // keys that some row of the tile sees
+    // this CTA's work, found once by warp 0
+    Span span;
+    int q0, rows;   // first query row within the sequence, rows of the tile (0: no work)
     int t0, n;      // its key tiles
     float ref[2][BM];      // R after the stream's last tile
     float odd_sum[BM];
@@ -352,24 +354,25 @@ struct TileTail {
 constexpr size_t kTileSmem = 1024 + kQBytes + 2 * STAGES * kKvBytes + sizeof(TileTail);
 static_assert(2 * (kTileSmem + 1024) <= 233472, "two CTAs an SM");
 
-// The sequence and tile of tile `index` of the packed batch: a warp walks the
-// offsets 256 sequences at a time, eight a lane. tile = -1 behind the last.
-__device__ __forceinline__ void find_tile(const Params& p, int index, int& seq, int& tile) {
+// The sequence (its rows, without the prefix) and tile of tile `index` of the
+// packed batch: a warp walks the offsets 256 sequences at a time, eight a lane,
+// so a chunk costs one round trip to memory. Returns the sequence, -1 behind
+// the last tile.
+__device__ __forceinline__ int find_tile(const Params& p, int index, int& begin, int& len,
+                                         int& tile) {
     const int lane = lane_id();
-    seq = -1, tile = 0;
-    long long total = 0;
+    int total = 0;
     for (int base = 0; base < p.batch; base += 256) {
-        int count[8], mine = 0;
         const int first = base + 8 * lane;
-        int prev = p.offsets[min(first, p.batch)];
+        int at[9];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int next = p.offsets[min(first + i + 1, p.batch)];
-            const int b = min(max(prev, 0), p.tokens), e = min(max(next, b), p.tokens);
-            count[i] = first + i < p.batch ? (e - b + BM - 1) / BM : 0;
-            mine += count[i];
-            prev = next;
-        }
+        for (int i = 0; i < 9; ++i) at[i] = p.offsets[min(first + i, p.batch)];
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < 9; ++i) at[i] = min(max(at[i], 0), p.tokens);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (first + i < p.batch) mine += (max(at[i + 1] - at[i], 0) + BM - 1) / BM;
         int upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -379,16 +382,23 @@ __device__ __forceinline__ void find_tile(const Params& p, int index, int& seq, 
         const unsigned past = __ballot_sync(0xFFFFFFFFu, total + upto > index);
         if (past != 0) {
             const int owner = __ffs(past) - 1;
-            int left = static_cast<int>(index - total) - (upto - mine), s = first;
+            int left = index - total - (upto - mine), s = 0, b = 0, n = 0;
+            bool found = false;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (s == first + i && left >= count[i]) left -= count[i], ++s;
-            seq = min(__shfl_sync(0xFFFFFFFFu, s, owner), p.batch - 1);
-            tile = max(__shfl_sync(0xFFFFFFFFu, left, owner), 0);
-            return;
+            for (int i = 0; i < 8; ++i) {
+                const int rows = first + i < p.batch ? max(at[i + 1] - at[i], 0) : 0;
+                const int count = (rows + BM - 1) / BM;
+                if (!found && left < count) found = true, s = first + i, b = at[i], n = rows;
+                if (!found) left -= count;
+            }
+            begin = __shfl_sync(0xFFFFFFFFu, b, owner);
+            len = __shfl_sync(0xFFFFFFFFu, n, owner);
+            tile = __shfl_sync(0xFFFFFFFFu, left, owner);
+            return __shfl_sync(0xFFFFFFFFu, found ? s : -1, owner);
         }
         total += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
+    return -1;
 }
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
@@ -477,42 +487,42 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     pdl_wait();
     if (warp == 0) {
         __syncwarp();
-        const int unit = static_cast<int>(blockIdx.x) / p.splits;
-        const int split = static_cast<int>(blockIdx.x) % p.splits;
-        int seq, tile;
+        const int unit = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.splits));
+        const unsigned split = blockIdx.x - static_cast<unsigned>(unit) * p.splits;
+        Span q{};
+        int tile = 0, rows = 0, q0 = 0, first = 0, count = 0;
         if (p.chunks > 0) {
-            seq = unit / p.chunks, tile = unit % p.chunks;
+            q = span_of(p, unit / p.chunks);
+            tile = unit % p.chunks;
         } else {
-            find_tile(p, unit, seq, tile);
+            int begin = 0;
+            const int seq = find_tile(p, unit, begin, q.len, tile);
+            q.begin = begin;
+            if (seq < 0) q.len = 0;
+            else if (p.mask == BL_MASK_PREFIX) q.prefix = min(max(p.prefix[seq], 0), q.len);
         }
-        if (seq >= 0) {
-            const Span q = span_of(p, seq);
-            const int tiles = (q.len - q.first + BM - 1) / BM;
-            if (tile >= tiles) {
-                seq = -1;
-            } else {
-                // with a causal mask the last rows see most: they start first
-                if (p.mask != BL_MASK_NONE) tile = tiles - 1 - tile;
-                const int q0 = q.first + tile * BM;
-                const int rows = min(q.len - q0, BM);
-                const int keys = visible(p, q, q0 + rows - 1);
-                const int nt = (keys + BN - 1) / BN;
-                const int t0 = static_cast<int>(1ll * nt * split / p.splits);
-                if (lane == 0) {
-                    tail->q0 = q0, tail->rows = rows, tail->keys = keys;
-                    tail->t0 = t0;
-                    tail->n = static_cast<int>(1ll * nt * (split + 1) / p.splits) - t0;
-                }
-            }
+        const int tiles = (q.len - q.first + BM - 1) / BM;
+        if (tile >= 0 && tile < tiles) {
+            // with a causal mask the last rows see most: they start first
+            if (p.mask != BL_MASK_NONE) tile = tiles - 1 - tile;
+            q0 = q.first + tile * BM;
+            rows = min(q.len - q0, BM);
+            // below 2^25 tiles and at most 8 splits: 32 bits hold the products
+            const unsigned nt = (visible(p, q, q0 + rows - 1) + BN - 1) / BN;
+            first = static_cast<int>(nt * split / p.splits);
+            count = static_cast<int>(nt * (split + 1) / p.splits) - first;
         }
-        if (lane == 0) tail->seq = seq;
+        if (lane == 0) {
+            tail->span = q;
+            tail->q0 = q0, tail->rows = rows, tail->t0 = first, tail->n = count;
+        }
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tail->tmem_base;
-    const int seq = tail->seq;
-    if (seq < 0) {  // no such tile (the same for every CTA of a cluster)
+    if (tail->rows == 0) {  // no such tile (the same for every CTA of a cluster)
         if (warp == 1) tmem_dealloc(tmem, kTmemCols);
         return;
     }
@@ -529,24 +539,24 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     };
     if (warp == 0) {
         // ------------------------------------------------------ producer
-        const int row0 = static_cast<int>(span_of(p, seq).begin);
+        const int row0 = static_cast<int>(tail->span.begin);
         if (elected && n > 0) {
             mbar_arrive_expect_tx(smem_u32(&tail->q_full), kQBytes);
             tma_load_2d(smem_u32(sQ), &tm_q, head * HD, row0 + tail->q0, smem_u32(&tail->q_full));
         }
         int loaded = 0;
-        for (int i = 0, s = 0, phase = 1; i < n; ++i) {
-            if (i >= STAGES && !wait_warp(&tail->kv_empty[s], phase, ST_TIMEOUT_TMA, i)) break;
-            const uint32_t bar = smem_u32(&tail->kv_full[s]);
-            const int y = row0 + (t0 + i) * BN;
+        for (int s = 0, phase = 1; loaded < n; ++loaded) {
+            if (loaded >= STAGES && !wait_warp(&tail->kv_empty[s], phase, ST_TIMEOUT_TMA, loaded))
+                break;
             if (elected) {
+                const uint32_t bar = smem_u32(&tail->kv_full[s]);
+                const int y = row0 + (t0 + loaded) * BN;
                 mbar_arrive_expect_tx(bar, 2 * kKvBytes);
                 tma_load_2d(smem_u32(sK + s * kKvBytes), &tm_kv, (p.heads + kvh) * HD, y, bar);
                 tma_load_2d(smem_u32(sV + s * kKvBytes), &tm_kv, (p.heads + p.kv_heads + kvh) * HD,
                             y, bar);
             }
             __syncwarp();
-            ++loaded;
             if (++s == STAGES) s = 0, phase ^= 1;
         }
         if (elected && n > 0 && *abort) {
@@ -567,7 +577,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         // operand, one swizzle atom wide, groups of 8 keys 1024 bytes apart
         const uint64_t dv = sdesc_sw128(smem_u32(sV), kKvBytes, 1024);
         constexpr uint64_t kStep = kKvBytes >> 4;
-        const int end = span_of(p, seq).len;
+        const int end = tail->span.len;
         // ring places, stepped as the loop goes: S runs SBUFS tiles ahead of PV
         int sb = 0, st = 0, st_phase = 0;  // of the next S: TMEM buffer, stage
         int pb = 0, p_phase = 0, pt = 0;   // of the next PV
@@ -645,7 +655,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         const int row = sub * 32 + lane;
         const uint32_t t_lane = tmem + (static_cast<uint32_t>(sub * 32) << 16);
         const uint32_t o_col = t_lane + kColO;
-        const Span q = span_of(p, seq);
+        const Span q = tail->span;
         const int at = tail->q0 + row;  // this row within the sequence
         const bool live = row < tail->rows;
         const int seen = live ? visible(p, q, at) : 0;
@@ -688,6 +698,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             if (!ok) break;
             tc_fence_after();
             const int valid = seen - k0;
+            // some row of the warp sees less than the whole tile
+            const bool cut = __any_sync(kFull, valid < BN);
             const float rel = static_cast<float>(at - k0);
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -715,7 +727,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                         s[e] = __float_as_uint(t);
                     }
                 }
-                if (valid < 32 * h + 32) {
+                if (cut) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (32 * h + e >= valid) s[e] = __float_as_uint(-INFINITY);
@@ -776,7 +788,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 uint32_t s[32];
                 tmem_ld32(s_col + 32 * h, s);
                 tmem_wait_ld();
-                if (kPlain && valid < 32 * h + 32) {
+                if (kPlain && cut) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (32 * h + e >= valid) s[e] = __float_as_uint(-INFINITY);
@@ -857,28 +869,42 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         cluster_sync();
         const int me = static_cast<int>(cluster_rank());
         const int r0 = BM * me / p.splits, r1 = min(BM * (me + 1) / p.splits, tail->rows);
-        const Span q = span_of(p, seq);
-        for (int i = r0 * 16 + threadIdx.x; i < r1 * 16; i += kTileThreads) {
+        const long long to = (tail->span.begin + tail->q0) * p.out_row + head * HD;
+        // (the loop's bound is the warp's, so that the warp reaches the cluster
+        // barrier after it as one)
+        for (int w0 = r0 * 16 + 32 * warp; w0 < r1 * 16; w0 += kTileThreads) {
+            const int i = min(w0 + lane, r1 * 16 - 1);  // the last lanes repeat a store
             const int row = i >> 4, k = i & 15;
+            const uint32_t at_ml = smem_u32(sV) + row * 8;
+            const uint32_t at_o = smem_u32(sK) + (row * 16 + (k ^ (row & 15))) * 16;
+            float2 ml[8];
+            float4 o[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s)  // every load on its way before the first use
+                if (s < p.splits) {
+                    ml[s] = dsmem_ld2(dsmem_addr(at_ml, s));
+                    o[s] = dsmem_ld4(dsmem_addr(at_o, s));
+                }
             float top = -INFINITY;
-            for (int s = 0; s < p.splits; ++s)
-                top = fmaxf(top, dsmem_ld2(dsmem_addr(smem_u32(sV) + row * 8, s)).x);
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s < p.splits) top = fmaxf(top, ml[s].x);
             const float ref = top == -INFINITY ? 0.0f : top;
             float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float sum = 0.0f;
-            for (int s = 0; s < p.splits; ++s) {
-                const float2 ml = dsmem_ld2(dsmem_addr(smem_u32(sV) + row * 8, s));
-                const float w = ex2(ml.x - ref);
-                const float4 v = dsmem_ld4(
-                    dsmem_addr(smem_u32(sK) + (row * 16 + (k ^ (row & 15))) * 16, s));
-                sum = fmaf(w, ml.y, sum);
-                a.x = fmaf(w, v.x, a.x), a.y = fmaf(w, v.y, a.y);
-                a.z = fmaf(w, v.z, a.z), a.w = fmaf(w, v.w, a.w);
-            }
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s < p.splits) {
+                    const float w = ex2(ml[s].x - ref);
+                    sum = fmaf(w, ml[s].y, sum);
+                    a.x = fmaf(w, o[s].x, a.x), a.y = fmaf(w, o[s].y, a.y);
+                    a.z = fmaf(w, o[s].z, a.z), a.w = fmaf(w, o[s].w, a.w);
+                }
             const float inv = 1.0f / sum;
-            store4(p.out, (q.begin + tail->q0 + row) * p.out_row + head * HD + 4 * k, p.out_dtype,
+            store4(p.out, to + row * p.out_row + 4 * k, p.out_dtype,
                    make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
         }
+        __syncwarp();
         cluster_sync();  // no CTA leaves while its part is read
     }
     tc_fence_before();
