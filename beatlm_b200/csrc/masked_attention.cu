@@ -70,219 +70,314 @@ __device__ __forceinline__ int visible(const Params& p, const Span& q, int i) {
     return p.mask == BL_MASK_NONE ? q.len : max(i + 1, q.prefix);
 }
 
-__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
-    if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+// Scores are kept in log2 units. A capped one, cap tanh(s / cap), is formed as
+// cap - 2 cap / (1 + e^(2 s / cap)): an absolute error of a few 2^-23 cap,
+// which is what an exponent needs, from two approximate functions; it goes to
+// +-cap at the ends without a branch.
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
-__device__ __forceinline__ void unpack8(const uint4& v, bool bf16, float (&f)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 t = unpack2(w[i], bf16);
-        f[2 * i] = t.x, f[2 * i + 1] = t.y;
-    }
-}
-
-// cap tanh(s / cap) as cap - 2 cap / (1 + e^(2 s / cap)): an absolute error of
-// a few 2^-23 cap, which is what an exponent needs.
-__device__ __forceinline__ float capped(float s, float cap, float two_log2e_over_cap) {
-    return cap - __fdividef(2.0f * cap, 1.0f + ex2(s * two_log2e_over_cap));
+__device__ __forceinline__ float sqrt_approx(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // ------------------------------------------------------------------ few rows
 //
-// One CTA computes R query rows of one K/V head (rows and heads of its group
-// alike) over one split of the keys. Eight lanes hold one key's 64 values, 8
-// each, so a warp reads four keys with one 16-byte load a lane and a score is
-// eight products a lane and three shuffles. Every group of eight lanes keeps
-// its own running maximum, sum and output over the keys it has seen; they are
-// merged once at the end: lanes, warps, then the cluster's CTAs.
-constexpr int kWarps = 8;
-constexpr int kUnroll = 4;  // key quads a warp has in flight
+// The newest rows of a stream: up to 16 query rows of one K/V head (rows and
+// heads of its group alike), for which the keys' bytes are what counts. Each
+// of a CTA's four warps walks its own 16-key tiles of one split of the keys,
+// with three tiles on their way to a shared-memory ring of its own (12 KB a
+// warp in flight, 12 warps an SM; no barrier between warps). 16 rows are the
+// smallest tile of the warp-level tensor instruction (m16n8k16), which takes
+// S = Q K^T and O += P V of a tile in 16 instructions, so the arithmetic stays
+// below the bytes: on the FMA units one row alone cost 400 instructions a
+// tile. Scores, maxima, sums and O are f32, P is rounded to f16 (it is at most
+// 1: the running maximum is exact here). Warps, then the cluster's CTAs, are
+// merged once at the end, in rank order.
+// MEASURED_TOKEN
+constexpr int kRowWarps = 4;
+constexpr int kRowTile = 16;    // keys of a tile
+constexpr int kRowStages = 4;
+constexpr int kMaxRows = 16;    // query rows of a CTA
+constexpr int kRowTileBytes = 2 * kRowTile * HD * 2;  // K, then V
+constexpr size_t kRowSmem = kRowWarps * kRowStages * kRowTileBytes;
+static_assert(kRowStages * kRowTileBytes >= kMaxRows * HD * 4, "a warp's O over its ring");
 
-template <int R>
-__global__ void __launch_bounds__(32 * kWarps) rows_kernel(const Params p, int bf16) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+    // past the split's keys nothing is read and zeros are written
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(real ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (kBf16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+                     "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+                     "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <bool kBf16>
+__global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_constant__ Params p) {
     pdl_trigger();
     pdl_wait();
-    __shared__ float part_o[kWarps][R][HD];
-    __shared__ float2 part_ml[kWarps][R];
-    __shared__ float cta_o[R][HD];
-    __shared__ float2 cta_ml[R];
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ float2 part_ml[kRowWarps][kMaxRows];
+    __shared__ float cta_o[kMaxRows][HD];
+    __shared__ float2 cta_ml[kMaxRows];
+    constexpr unsigned kFull = 0xFFFFFFFFu;
     const int warp = warp_id(), lane = lane_id();
-    const int split = blockIdx.x % p.splits;
-    const int unit = blockIdx.x / p.splits;
-    const int chunk = unit % p.chunks;
+    const int split = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.splits));
+    const int unit = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.splits));
+    const int c0 = unit % p.chunks * kMaxRows;
     const Span q = span_of(p, unit / p.chunks);
-    const int nrows = q.len - q.first;
     const int kvh = blockIdx.y;
-    const int c0 = chunk * R;
-    if (c0 >= nrows * p.group) return;  // the whole cluster leaves
+    const int rows = min((q.len - q.first) * p.group - c0, kMaxRows);
+    if (rows <= 0) return;  // the whole cluster leaves
 
-    const int g = lane >> 3, d = (lane & 7) * 8;
-    float qv[R][8], acc[R][8], m[R], l[R], slope[R], qp[R][3];
-    int row[R], seen[R], most = 0;
-    for (int r = 0; r < R; ++r) {
-        const int c = min(c0 + r, nrows * p.group - 1);
+    // This thread's two query rows (of the 16: g and g + 8), as the products'
+    // accumulators hold them; a row past the last repeats it and is not stored.
+    const int g = lane >> 2, quad = lane & 3;
+    int row[2], seen[2];
+    float slope[2], qp[2][3];
+    uint32_t qa[HD / 16][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int c = c0 + min(g + 8 * r, rows - 1);
         const int head = kvh * p.group + c % p.group;
         row[r] = q.first + c / p.group;
         seen[r] = visible(p, q, row[r]);
-        most = max(most, seen[r]);
-        const uint4 v = *reinterpret_cast<const uint4*>(p.qkv + (q.begin + row[r]) * p.row +
-                                                        head * HD + d);
-        unpack8(v, bf16 != 0, qv[r]);
-        for (int i = 0; i < 8; ++i) qv[r][i] *= p.scale, acc[r][i] = 0.0f;
-        m[r] = -INFINITY, l[r] = 0.0f;
-        slope[r] = p.slopes != nullptr ? p.slopes[head] : 0.0f;
+        slope[r] = p.slopes != nullptr ? p.slopes[head] * kLog2e : 0.0f;
+        const uint16_t* src = p.qkv + (q.begin + row[r]) * p.row + head * HD + 2 * quad;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+            qa[k][r] = *reinterpret_cast<const uint32_t*>(src + 16 * k);
+            qa[k][r + 2] = *reinterpret_cast<const uint32_t*>(src + 16 * k + 8);
+        }
+#pragma unroll
         for (int a = 0; a < 3; ++a)
             qp[r][a] = p.pos != nullptr && a < p.pos_axes
                            ? p.pos[(q.begin + row[r]) * p.pos_row + a] : 0.0f;
     }
-    const float cap_in = p.cap > 0.0f ? 2.0f * kLog2e / p.cap : 0.0f;
-    const int per = ((most + p.splits - 1) / p.splits + 15) / 16 * 16;
-    const int k0 = min(split * per, most), k1 = min(k0 + per, most);
-    const uint16_t* kbase = p.qkv + q.begin * p.row + (p.heads + kvh) * HD + d;
-    const uint16_t* vbase = kbase + p.kv_heads * HD;
+    const int most = visible(p, q, q.first + (c0 + rows - 1) / p.group);  // of the last row
+    const int tiles = (most + kRowTile - 1) / kRowTile;
+    const int first = static_cast<int>(static_cast<unsigned>(tiles) * split / p.splits);
+    const int last = static_cast<int>(static_cast<unsigned>(tiles) * (split + 1) / p.splits);
 
-    for (int base = k0 + 4 * kUnroll * warp; base < k1; base += 4 * kUnroll * kWarps) {
-        uint4 kr[kUnroll], vr[kUnroll];
+    const uint16_t* kbase = p.qkv + q.begin * p.row + (p.heads + kvh) * HD + (lane & 7) * 8;
+    const long long to_v = static_cast<long long>(p.kv_heads) * HD;
+    const uint32_t mine = smem_u32(ring) + warp * kRowStages * kRowTileBytes;
+    auto fetch = [&](int tile, int stage) {
+        if (tile < last) {
+            const uint32_t dst = mine + stage * kRowTileBytes;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int key = base + 4 * u + g;
-            kr[u] = vr[u] = make_uint4(0, 0, 0, 0);
-            if (key < k1) {
-                kr[u] = *reinterpret_cast<const uint4*>(kbase + key * p.row);
-                vr[u] = *reinterpret_cast<const uint4*>(vbase + key * p.row);
+            for (int i = 0; i < kRowTile / 4; ++i) {
+                const int k = 4 * i + (lane >> 3), key = tile * kRowTile + k;
+                // a key row is 128 bytes: its eight 16-byte parts rotated by
+                // the row, so that the matrix loads meet no bank twice
+                const uint32_t at = dst + k * 128 + (((lane & 7) ^ (k & 7)) << 4);
+                const uint16_t* src = kbase + min(key, most - 1) * p.row;
+                cp_async16(at, src, key < most);
+                cp_async16(at + kRowTile * 128, src + to_v, key < most);
             }
         }
-        float s[R][kUnroll];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float o[HD / 8][4];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float kf[8];
-            unpack8(kr[u], bf16 != 0, kf);
-            const int key = base + 4 * u + g;
-            float kp[3] = {0.0f, 0.0f, 0.0f};
-            if (p.pos != nullptr && key < k1)
-                for (int a = 0; a < p.pos_axes; ++a) kp[a] = p.pos[(q.begin + key) * p.pos_row + a];
+    for (int d = 0; d < HD / 8; ++d)
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float t = 0.0f;
+        for (int e = 0; e < 4; ++e) o[d][e] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const bool capped_scores = p.cap > 0.0f;
+    const float in = capped_scores ? 2.0f * p.scale / p.cap * kLog2e : p.scale * kLog2e;
+    const float cap2 = p.cap * kLog2e;
+
+    for (int i = 0; i < kRowStages - 1; ++i) fetch(first + warp + i * kRowWarps, i);
+    int stage = 0;
+    for (int tile = first + warp; tile < last; tile += kRowWarps) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 2) : "memory");
+        __syncwarp();
+        // the stage read last time is free: every lane is past it
+        fetch(tile + (kRowStages - 1) * kRowWarps, (stage + kRowStages - 1) % kRowStages);
+        const uint32_t sk = mine + stage * kRowTileBytes, sv = sk + kRowTile * 128;
+        stage = (stage + 1) % kRowStages;
+        const int base = tile * kRowTile;
+        float s[2][4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t = fmaf(qv[r][i], kf[i], t);
-                t += __shfl_xor_sync(0xFFFFFFFFu, t, 1);
-                t += __shfl_xor_sync(0xFFFFFFFFu, t, 2);
-                t += __shfl_xor_sync(0xFFFFFFFFu, t, 4);
-                if (p.cap > 0.0f) t = capped(t, p.cap, cap_in);
-                if (p.slopes != nullptr) {
-                    float far;
-                    if (p.pos != nullptr) {
-                        const float x = qp[r][0] - kp[0], y = qp[r][1] - kp[1], z = qp[r][2] - kp[2];
-                        far = sqrtf(fmaf(x, x, fmaf(y, y, z * z)));
-                    } else {
-                        far = fabsf(static_cast<float>(row[r] - key));
-                    }
-                    t = fmaf(-slope[r], far, t);
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+            // keys 0..7 and 8..15 by the two halves of 16 columns
+            uint32_t b[4];
+            const int key = (lane >> 4) * 8 + (lane & 7), part = 2 * k + ((lane >> 3) & 1);
+            ldmatrix4(sk + key * 128 + ((part ^ (key & 7)) << 4), b);
+            mma16<kBf16>(s[0], qa[k], b[0], b[1]);
+            mma16<kBf16>(s[1], qa[k], b[2], b[3]);
+        }
+        // s[t][2 r + e]: query row g + 8 r, key base + 8 t + 2 quad + e
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int key = base + 8 * t + 2 * quad + e;
+                float kp[3] = {0.0f, 0.0f, 0.0f};
+                if (p.pos != nullptr) {
+#pragma unroll
+                    for (int a = 0; a < 3; ++a)
+                        if (key < most && a < p.pos_axes) kp[a] = p.pos[(q.begin + key) * p.pos_row + a];
                 }
-                s[r][u] = key < min(k1, seen[r]) ? t * kLog2e : -INFINITY;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float x = s[t][2 * r + e] * in;
+                    if (capped_scores) x = fmaf(rcp_approx(1.0f + ex2(x)), -2.0f * cap2, cap2);
+                    if (p.slopes != nullptr) {
+                        float far = fabsf(static_cast<float>(row[r] - key));
+                        if (p.pos != nullptr) {
+                            const float dx = qp[r][0] - kp[0], dy = qp[r][1] - kp[1],
+                                        dz = qp[r][2] - kp[2];
+                            far = sqrt_approx(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
+                        }
+                        x = fmaf(-slope[r], far, x);
+                    }
+                    x = key < seen[r] ? x : -INFINITY;
+                    s[t][2 * r + e] = x;
+                    top[r] = fmaxf(top[r], x);
+                }
+            }
+        uint32_t pa[4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            top[r] = fmaxf(top[r], __shfl_xor_sync(kFull, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(kFull, top[r], 2));
+            top[r] = fmaxf(top[r], m[r]);
+        }
+        if (__any_sync(kFull, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float shrink = ex2(m[r] - (top[r] == -INFINITY ? 0.0f : top[r]));
+                m[r] = top[r];
+                l[r] *= shrink;
+#pragma unroll
+                for (int d = 0; d < HD / 8; ++d) o[d][2 * r] *= shrink, o[d][2 * r + 1] *= shrink;
             }
         }
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float top = m[r];
+        for (int r = 0; r < 2; ++r) {
+            const float ref = m[r] == -INFINITY ? 0.0f : m[r];  // no key seen yet
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, s[r][u]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            const float shrink = ex2(m[r] - ref);
-            m[r] = top;
-            l[r] *= shrink;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[r][i] *= shrink;
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) s[r][u] = ex2(s[r][u] - ref), l[r] += s[r][u];
+            for (int t = 0; t < 2; ++t) {
+                const float a = ex2(s[t][2 * r] - ref), b = ex2(s[t][2 * r + 1] - ref);
+                l[r] += a + b;
+                pa[2 * t + r] = pack_f16x2(a, b);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float vf[8];
-            unpack8(vr[u], false, vf);
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[r][i] = fmaf(s[r][u], vf[i], acc[r][i]);
+        for (int d = 0; d < HD / 16; ++d) {
+            // keys 0..7 and 8..15 of columns 16 d..16 d + 7, then of the next 8
+            uint32_t b[4];
+            const int key = lane & 15, part = 2 * d + (lane >> 4);
+            ldmatrix4_trans(sv + key * 128 + ((part ^ (key & 7)) << 4), b);
+            mma16<false>(o[2 * d], pa, b[0], b[1]);
+            mma16<false>(o[2 * d + 1], pa, b[2], b[3]);
         }
     }
-
-    // lanes of one key group -> warp
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    // the warp's sums, and its O over its ring
+    float* po = reinterpret_cast<float*>(ring + warp * kRowStages * kRowTileBytes);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const float top = fmaxf(fmaxf(m[r], __shfl_xor_sync(0xFFFFFFFFu, m[r], 8)),
-                                __shfl_xor_sync(0xFFFFFFFFu, fmaxf(m[r], __shfl_xor_sync(
-                                    0xFFFFFFFFu, m[r], 8)), 16));
-        const float w = ex2(m[r] - (top == -INFINITY ? 0.0f : top));
-        l[r] *= w;
-        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 8);
-        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 16);
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(kFull, l[r], 1);
+        l[r] += __shfl_xor_sync(kFull, l[r], 2);
+        if (quad == 0) part_ml[warp][g + 8 * r] = make_float2(m[r], l[r]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            acc[r][i] *= w;
-            acc[r][i] += __shfl_xor_sync(0xFFFFFFFFu, acc[r][i], 8);
-            acc[r][i] += __shfl_xor_sync(0xFFFFFFFFu, acc[r][i], 16);
-        }
-        if (g == 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) part_o[warp][r][d + i] = acc[r][i];
-            if (lane == 0) part_ml[warp][r] = make_float2(top, l[r]);
-        }
+        for (int d = 0; d < HD / 8; ++d)
+            *reinterpret_cast<float2*>(po + (g + 8 * r) * HD + 8 * d + 2 * quad) =
+                make_float2(o[d][2 * r], o[d][2 * r + 1]);
     }
     __syncthreads();
+    auto put = [&](int r, int e, float v) {
+        const int c = c0 + r;
+        const long long at = (q.begin + q.first + c / p.group) * p.out_row +
+                             (kvh * p.group + c % p.group) * HD + e;
+        if (p.out_dtype == BL_F32) static_cast<float*>(p.out)[at] = v;
+        else if (p.out_dtype == BL_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+    };
     // warps -> CTA
-    for (int t = threadIdx.x; t < R * HD; t += 32 * kWarps) {
+    for (int t = threadIdx.x; t < rows * HD; t += 32 * kRowWarps) {
         const int r = t / HD, e = t % HD;
-        float top = -INFINITY, o = 0.0f, sum = 0.0f;
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part_ml[w][r].x);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        for (int w = 0; w < kWarps; ++w) {
+        float best = -INFINITY, v = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) best = fmaxf(best, part_ml[w][r].x);
+        const float ref = best == -INFINITY ? 0.0f : best;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) {
             const float f = ex2(part_ml[w][r].x - ref);
-            o = fmaf(f, part_o[w][r][e], o);
+            v = fmaf(f, reinterpret_cast<const float*>(ring + w * kRowStages * kRowTileBytes)[r * HD + e], v);
             sum = fmaf(f, part_ml[w][r].y, sum);
         }
-        cta_o[r][e] = o;
-        if (e == 0) cta_ml[r] = make_float2(top, sum);
-    }
-    __syncthreads();
-    if (p.splits > 1) {
-        fence_cluster();
-        cluster_sync();
-    }
-    // CTAs -> row, by the cluster's first CTA
-    if (split == 0) {
-        for (int t = threadIdx.x; t < R * HD; t += 32 * kWarps) {
-            const int r = t / HD, e = t % HD;
-            const int c = c0 + r;
-            if (c >= nrows * p.group) continue;
-            float top = -INFINITY, o = 0.0f, sum = 0.0f;
-            for (int k = 0; k < p.splits; ++k)
-                top = fmaxf(top, dsmem_ld2(dsmem_addr(smem_u32(&cta_ml[r]), k)).x);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            for (int k = 0; k < p.splits; ++k) {
-                const float2 ml = dsmem_ld2(dsmem_addr(smem_u32(&cta_ml[r]), k));
-                const float f = ex2(ml.x - ref);
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v)
-                             : "r"(dsmem_addr(smem_u32(&cta_o[r][e]), k)));
-                o = fmaf(f, v, o);
-                sum = fmaf(f, ml.y, sum);
-            }
-            o = sum == 0.0f ? 0.0f : o / sum;
-            const long long at = (q.begin + q.first + c / p.group) * p.out_row +
-                                 (kvh * p.group + c % p.group) * HD + e;
-            if (p.out_dtype == BL_F32) static_cast<float*>(p.out)[at] = o;
-            else if (p.out_dtype == BL_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(o);
-            else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o);
+        if (p.splits == 1) {
+            put(r, e, v / sum);
+        } else {
+            cta_o[r][e] = v;
+            if (e == 0) cta_ml[r] = make_float2(best, sum);
         }
     }
-    if (p.splits > 1) {
-        __syncwarp();
-        cluster_sync();  // no CTA leaves while its partials are read
+    if (p.splits == 1) return;
+    __syncthreads();
+    fence_cluster();
+    cluster_sync();
+    // CTAs -> rows: the cluster's CTAs share out the values
+    for (int t = split * 32 * kRowWarps + threadIdx.x; t < rows * HD; t += p.splits * 32 * kRowWarps) {
+        const int r = t / HD, e = t % HD;
+        float2 ml[8];
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)  // every load on its way before the first use
+            if (k < p.splits) {
+                ml[k] = dsmem_ld2(dsmem_addr(smem_u32(&cta_ml[r]), k));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[k])
+                             : "r"(dsmem_addr(smem_u32(&cta_o[r][e]), k)));
+            }
+        float best = -INFINITY, total = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < p.splits) best = fmaxf(best, ml[k].x);
+        const float ref = best == -INFINITY ? 0.0f : best;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < p.splits) {
+                const float f = ex2(ml[k].x - ref);
+                total = fmaf(f, v[k], total);
+                sum = fmaf(f, ml[k].y, sum);
+            }
+        put(r, e, total / sum);
     }
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while its part is read
 }
 
 // ------------------------------------------------------------------ tiles
@@ -406,17 +501,6 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ float rcp_approx(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float sqrt_approx(float x) {
-    float y;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ void store4(void* out, long long at, int dt, const float4& v) {
     if (dt == BL_F32) {
         *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
@@ -995,25 +1079,25 @@ Params params_of(const bl_masked_attention_args& a) {
 
 int prepare_rows(const bl_masked_attention_args& a, Launch* out) {
     Params p = params_of(a);
-    const uint64_t rows = p.last_rows > 0 ? p.last_rows : p.tokens;
-    const uint64_t combos = rows * p.group;
-    const int r = combos <= 1 ? 1 : combos <= 2 ? 2 : 4;
-    p.chunks = static_cast<int>((combos + r - 1) / r);
-    const uint64_t units = 1ull * p.chunks * a.batch;
-    const uint64_t ctas = units * p.kv_heads;
+    const uint64_t combos = 1ull * p.last_rows * p.group;
+    p.chunks = static_cast<int>((combos + kMaxRows - 1) / kMaxRows);
+    const uint64_t units = 1ull * p.chunks * a.batch, ctas = units * p.kv_heads;
+    // Splits: enough CTAs for three an SM twice over (sequences differ in
+    // length), each with 256 keys at least. MEASURED_SPLITS
     p.splits = a.key_splits ? static_cast<int>(a.key_splits)
                             : static_cast<int>(std::max<uint64_t>(
-                                  1, std::min<uint64_t>({8, 296 / ctas, (a.tokens + 255ull) / 256})));
+                                  1, std::min<uint64_t>({8, (888 + ctas - 1) / ctas, a.tokens / 256})));
     if (units * p.splits > 0x7FFFFFFFull)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: grid too large");
-    auto kern = r == 1 ? rows_kernel<1> : r == 2 ? rows_kernel<2> : rows_kernel<4>;
+    auto kern = a.qk_dtype == BL_BF16 ? rows_kernel<true> : rows_kernel<false>;
+    BL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(kRowSmem)));
     const dim3 grid(static_cast<unsigned>(units * p.splits), p.kv_heads);
-    const int bf16 = a.qk_dtype == BL_BF16;
     out->op = BL_OP_MASKED_ATTENTION;
     out->run = [=](cudaStream_t s) {
-        return p.splits > 1 ? launch_k_cluster(kern, grid, dim3(32 * kWarps), dim3(p.splits, 1, 1),
-                                               0, s, p, bf16)
-                            : launch_k(kern, grid, dim3(32 * kWarps), 0, s, p, bf16);
+        return p.splits > 1 ? launch_k_cluster(kern, grid, dim3(32 * kRowWarps),
+                                               dim3(p.splits, 1, 1), kRowSmem, s, p)
+                            : launch_k(kern, grid, dim3(32 * kRowWarps), kRowSmem, s, p);
     };
     return BL_OK;
 }
@@ -1074,12 +1158,11 @@ int prepare_tiles(const bl_masked_attention_args& a, Launch* out) {
 int prepare_masked_attention(const bl_masked_attention_args& a, Launch* out) {
     const int rc = masked::validate(a);
     if (rc != BL_OK) return rc;
-    // The last rows of a stream: while a K/V head's query rows are few, the
-    // tensor cores' 128-row tile would be nearly empty and the keys' bytes
-    // are what counts.
+    // The last rows of a stream: while a K/V head's query rows are few, a
+    // 128-row tile would be nearly empty and the keys' bytes are what counts.
     const uint32_t kv = a.kv_heads ? a.kv_heads : a.heads;
     const uint64_t combos = 1ull * std::min(a.last_rows, a.tokens) * (a.heads / kv);
-    return a.last_rows > 0 && combos <= 4 ? masked::prepare_rows(a, out)
+    return a.last_rows > 0 && combos <= masked::kMaxRows ? masked::prepare_rows(a, out)
                                           : masked::prepare_tiles(a, out);
 }
 

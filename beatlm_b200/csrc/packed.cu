@@ -96,8 +96,7 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const int* grids, const 
 struct RopeParams {
     long long rows;
     int heads, head_dim, pairs;
-    int axes, sections[3];  // pairs of each axis
-    int pairing;            // BL_ROPE_*
+    int sections[3];  // pairs of each axis, 0 past the last
     int inverse;
     const void* x;
     long long x_stride;
@@ -105,6 +104,9 @@ struct RopeParams {
     long long out_stride;
     const float* pos;
     long long pos_stride;
+    // the block's shape: chunks of a head's pairs, head groups, rows, and the
+    // heads a thread turns one after the other
+    int chunks, groups, tile_rows, per_thread;
     double turn[BL_ROPE_MAX_PAIRS];  // frequency / pi: angles in half turns
 };
 
@@ -117,54 +119,147 @@ template <> __device__ __forceinline__ float down(float v) { return v; }
 template <> __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 
-// One block a row: its angles' cosines and sines once, in shared memory, then
-// every head's pairs. The angle is formed in 64 bits in half turns and reduced
-// to [-1, 1] before the 32-bit sincospif, so positions of 10^6 and more lose
-// nothing that the result could hold.
-template <typename T>
+template <typename T, int kVec>
+struct alignas(sizeof(T) * kVec) Vec {
+    T v[kVec];
+};
+
+// A block turns tiles of rows, each thread kVec neighbouring pairs of several
+// heads: two vectors of a head (its halves, an axis's halves, or neighbours),
+// so every global access is a whole vector and a warp's cover whole sectors.
+// What bounds it is memory: each value read once and written once. The angles
+// are few beside the values (one a row and pair, against one pair a head), but
+// dear: formed in 64 bits in half turns and reduced to [-1, 1] before the
+// 32-bit sincospif, so that positions of 10^6 and more lose nothing the result
+// could hold. A tile's cosines and sines are made once, into one of two shared
+// tables (so one barrier a tile is enough), while the tile's values are on
+// their way; a thread keeps the frequency of its pair over all its tiles.
+// 60280 rows x 32 heads x 64 in bf16 (494 MB): MEASURED_ROPE.
+constexpr int kRopeBatch = 4;  // heads a thread has in flight
+
+template <typename T, int kVec, int kPairing>
 __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeParams p) {
     pdl_trigger();
     pdl_wait();
-    __shared__ float cs[BL_ROPE_MAX_PAIRS], sn[BL_ROPE_MAX_PAIRS];
-    const long long r = blockIdx.x;
-    const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
-    T* y = static_cast<T*>(p.out) + r * p.out_stride;
-    for (int j = threadIdx.x; j < p.pairs; j += 256) {
-        const int a = j < p.sections[0] ? 0 : j < p.sections[0] + p.sections[1] ? 1 : 2;
-        double h = static_cast<double>(p.pos[r * p.pos_stride + a]) * p.turn[j];
-        h -= 2.0 * rint(0.5 * h);
-        float s, c;
-        sincospif(static_cast<float>(h), &s, &c);
-        cs[j] = c, sn[j] = p.inverse ? -s : s;
+    extern __shared__ float table[];  // [2][tile_rows][2][pairs]
+    using V = Vec<T, kVec>;
+    const int t = threadIdx.x;
+    // as a maker of angles: pair t % pairs of every step-th row
+    const int step = 256 / p.pairs, pair = t % p.pairs, first_row = t / p.pairs;
+    const int axis = pair < p.sections[0] ? 0 : pair < p.sections[0] + p.sections[1] ? 1 : 2;
+    const double turn = p.turn[pair];
+    // as a turner of pairs: chunk, head group, row of the tile
+    const int chunk = t % p.chunks, group = t / p.chunks % p.groups;
+    const int row = t / (p.chunks * p.groups);
+    const int j = chunk * kVec;
+    int lo, hi;
+    if (kPairing == BL_ROPE_HALF) {
+        lo = j, hi = j + p.pairs;
+    } else if (kPairing == BL_ROPE_ADJACENT) {
+        lo = 2 * j, hi = lo + kVec;
+    } else {
+        const int s0 = p.sections[0], s1 = s0 + p.sections[1];
+        const int start = j < s0 ? 0 : j < s1 ? s0 : s1;
+        lo = start + j, hi = lo + (j < s0 ? s0 : j < s1 ? s1 - s0 : p.sections[2]);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.heads * p.pairs; i += 256) {
-        const int head = i / p.pairs, j = i - head * p.pairs;
-        int lo, hi;
-        if (p.pairing == BL_ROPE_HALF) {
-            lo = j, hi = j + p.pairs;
-        } else if (p.pairing == BL_ROPE_ADJACENT) {
-            lo = 2 * j, hi = lo + 1;
-        } else {
-            const int first = j < p.sections[0] ? 0
-                              : j < p.sections[0] + p.sections[1] ? p.sections[0]
-                                                                  : p.sections[0] + p.sections[1];
-            const int n = j < p.sections[0] ? p.sections[0]
-                          : j < p.sections[0] + p.sections[1] ? p.sections[1]
-                                                              : p.sections[2];
-            lo = first + j, hi = lo + n;
+    const int table_size = 2 * p.tile_rows * p.pairs;
+    const long long tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
+    int buffer = 0;
+    for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x, buffer ^= 1) {
+        const long long r0 = tile * p.tile_rows;
+        const long long r = r0 + row;
+        const bool mine = row < p.tile_rows && r < p.rows;
+        const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
+        T* y = static_cast<T*>(p.out) + r * p.out_stride;
+        V a[kRopeBatch], b[kRopeBatch];
+        auto load = [&](int base) {
+#pragma unroll
+            for (int i = 0; i < kRopeBatch; ++i) {
+                const int head = group + (base + i) * p.groups;
+                if (mine && base + i < p.per_thread && head < p.heads) {
+                    a[i] = *reinterpret_cast<const V*>(x + head * p.head_dim + lo);
+                    b[i] = *reinterpret_cast<const V*>(x + head * p.head_dim + hi);
+                }
+            }
+        };
+        load(0);
+        float* cs = table + buffer * table_size;
+        for (int k = first_row; k < p.tile_rows && first_row < step; k += step) {
+            if (r0 + k >= p.rows) break;
+            double h = static_cast<double>(p.pos[(r0 + k) * p.pos_stride + axis]) * turn;
+            h -= 2.0 * rint(0.5 * h);
+            float sn, cn;
+            sincospif(static_cast<float>(h), &sn, &cn);
+            cs[2 * k * p.pairs + pair] = cn;
+            cs[(2 * k + 1) * p.pairs + pair] = p.inverse ? -sn : sn;
         }
-        const long long b = static_cast<long long>(head) * p.head_dim;
-        const float u = up(x[b + lo]), v = up(x[b + hi]);
-        y[b + lo] = down<T>(u * cs[j] - v * sn[j]);
-        y[b + hi] = down<T>(v * cs[j] + u * sn[j]);
+        __syncthreads();
+        if (mine) {
+            float c[kVec], s[kVec];
+            const float* at = cs + 2 * row * p.pairs + j;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) c[e] = at[e], s[e] = at[p.pairs + e];
+            for (int base = 0; base < p.per_thread; base += kRopeBatch) {
+                if (base > 0) load(base);
+#pragma unroll
+                for (int i = 0; i < kRopeBatch; ++i) {
+                    const int head = group + (base + i) * p.groups;
+                    if (base + i >= p.per_thread || head >= p.heads) continue;
+                    V u, w;
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) {
+                        // pair e of the chunk: element e of each vector, or
+                        // for neighbours the vectors' elements 2 e, 2 e + 1
+                        if (kPairing != BL_ROPE_ADJACENT) {
+                            const float f = up(a[i].v[e]), g = up(b[i].v[e]);
+                            u.v[e] = down<T>(f * c[e] - g * s[e]);
+                            w.v[e] = down<T>(g * c[e] + f * s[e]);
+                        } else if (kVec == 1) {
+                            const float f = up(a[i].v[0]), g = up(b[i].v[0]);
+                            u.v[0] = down<T>(f * c[0] - g * s[0]);
+                            w.v[0] = down<T>(g * c[0] + f * s[0]);
+                        } else {
+                            const V& in = 2 * e < kVec ? a[i] : b[i];
+                            V& to = 2 * e < kVec ? u : w;
+                            const int k = 2 * e % kVec;
+                            const float f = up(in.v[k]), g = up(in.v[(k + 1) % kVec]);
+                            to.v[k] = down<T>(f * c[e] - g * s[e]);
+                            to.v[(k + 1) % kVec] = down<T>(g * c[e] + f * s[e]);
+                        }
+                    }
+                    *reinterpret_cast<V*>(y + head * p.head_dim + lo) = u;
+                    *reinterpret_cast<V*>(y + head * p.head_dim + hi) = w;
+                }
+            }
+        }
+        const int rest = p.head_dim - 2 * p.pairs;  // values that do not turn
+        if (rest > 0 && p.x != p.out) {
+            const int per_row = p.heads * rest;
+            const int n = static_cast<int>(min(static_cast<long long>(p.tile_rows), p.rows - r0));
+            for (int k = 0; k < n; ++k) {
+                const T* from = static_cast<const T*>(p.x) + (r0 + k) * p.x_stride;
+                T* to = static_cast<T*>(p.out) + (r0 + k) * p.out_stride;
+                for (int i = t; i < per_row; i += 256) {
+                    const int e = i / rest * p.head_dim + 2 * p.pairs + i % rest;
+                    to[e] = from[e];
+                }
+            }
+        }
     }
-    const int rest = p.head_dim - 2 * p.pairs;  // elements that do not turn
-    if (rest > 0 && static_cast<const void*>(x) != static_cast<const void*>(y))
-        for (int i = threadIdx.x; i < p.heads * rest; i += 256) {
-            const long long e = static_cast<long long>(i / rest) * p.head_dim + 2 * p.pairs + i % rest;
-            y[e] = x[e];
-        }
+}
+
+using RopeKernel = void (*)(const RopeParams);
+template <typename T, int kVec>
+RopeKernel rope_of(int pairing) {
+    return pairing == BL_ROPE_HALF       ? rope_kernel<T, kVec, BL_ROPE_HALF>
+           : pairing == BL_ROPE_ADJACENT ? rope_kernel<T, kVec, BL_ROPE_ADJACENT>
+                                         : rope_kernel<T, kVec, BL_ROPE_AXIS_HALF>;
+}
+template <typename T>
+RopeKernel rope_of(int pairing, int vec) {
+    if constexpr (sizeof(T) == 2)
+        if (vec == 8) return rope_of<T, 8>(pairing);
+    return vec == 4 ? rope_of<T, 4>(pairing) : vec == 2 ? rope_of<T, 2>(pairing) : rope_of<T, 1>(pairing);
 }
 
 }  // namespace packed
@@ -255,9 +350,8 @@ int prepare_rope(const bl_rope_args& a, Launch* out) {
     }
     RopeParams p{};
     p.rows = a.rows, p.heads = static_cast<int>(a.heads), p.head_dim = static_cast<int>(a.head_dim);
-    p.pairs = static_cast<int>(pairs), p.axes = static_cast<int>(a.axes);
+    p.pairs = static_cast<int>(pairs), p.inverse = a.inverse != 0;
     for (uint32_t i = 0; i < a.axes; ++i) p.sections[i] = static_cast<int>(a.sections[i]);
-    p.pairing = a.pairing, p.inverse = a.inverse != 0;
     p.x = a.x, p.x_stride = static_cast<long long>(xs);
     p.out = a.out, p.out_stride = static_cast<long long>(os);
     p.pos = a.positions, p.pos_stride = static_cast<long long>(ps);
@@ -271,13 +365,34 @@ int prepare_rope(const bl_rope_args& a, Launch* out) {
             if (!std::isfinite(f)) return fail(BL_ERR_INVALID, "rope: frequency %d is not finite", j);
             p.turn[j] = f / 3.14159265358979323846;
         }
-    auto kern = a.dtype == BL_F32   ? packed::rope_kernel<float>
-                : a.dtype == BL_F16 ? packed::rope_kernel<__half>
-                                    : packed::rope_kernel<__nv_bfloat16>;
-    out->op = BL_OP_ROPE;
-    out->run = [=](cudaStream_t s) {
-        return launch_k(kern, dim3(static_cast<unsigned>(p.rows)), dim3(256), 0, s, p);
+    // The widest vectors (at most 16 bytes) that every chunk of pairs, head,
+    // row and base starts on a multiple of: a power of two that divides them
+    // all. 16-byte vectors take MEASURED_VEC.
+    int vec = static_cast<int>(16 / esz);
+    auto divides = [&](int v) {
+        bool ok = pairs % v == 0 && a.head_dim % v == 0 && xs % v == 0 && os % v == 0 &&
+                  px % (v * esz) == 0 && po % (v * esz) == 0;
+        if (a.pairing == BL_ROPE_AXIS_HALF)
+            for (uint32_t i = 0; i < a.axes; ++i) ok = ok && a.sections[i] % v == 0;
+        return ok;
     };
+    while (vec > 1 && !divides(vec)) vec /= 2;
+    p.chunks = p.pairs / vec;
+    // Heads a thread turns with one reading of its cosines: four where that
+    // leaves every SM its threads, else one, for the shortest way through.
+    const uint64_t work = 1ull * a.rows * a.heads * p.chunks;
+    const int want = work >= 4ull * 148 * 2048 ? packed::kRopeBatch : 1;
+    p.groups = std::max(1, std::min((p.heads + want - 1) / want, 256 / p.chunks));
+    p.per_thread = (p.heads + p.groups - 1) / p.groups;
+    p.tile_rows = std::max(1, 256 / (p.chunks * p.groups));
+    const uint64_t tiles = (a.rows + p.tile_rows - 1ull) / p.tile_rows;
+    const size_t smem = 4ull * p.tile_rows * p.pairs * sizeof(float);
+    const unsigned blocks = static_cast<unsigned>(std::min<uint64_t>(tiles, 148 * 8));
+    const packed::RopeKernel kern = a.dtype == BL_F32   ? packed::rope_of<float>(a.pairing, vec)
+                                    : a.dtype == BL_F16 ? packed::rope_of<__half>(a.pairing, vec)
+                                                        : packed::rope_of<__nv_bfloat16>(a.pairing, vec);
+    out->op = BL_OP_ROPE;
+    out->run = [=](cudaStream_t s) { return launch_k(kern, dim3(blocks), dim3(256), smem, s, p); };
     return BL_OK;
 }
 

@@ -271,33 +271,37 @@ MASK = {None: 0, "none": 0, "causal": 1, "prefix": 2}
 PAIRING = {"half": 0, "adjacent": 1, "axis_half": 2}
 
 
-def _check(what, t, dtype=None, rows=None):
-    """A CUDA tensor of `dtype` (None = any) whose last dimension is contiguous."""
-    if not t.is_cuda:
-        raise ValueError("%s: a CUDA tensor, not one on %s" % (what, t.device))
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError("%s: %s, not %s" % (what, dtype, t.dtype))
-    if t.numel() and t.stride(-1) != 1:
-        raise ValueError("%s: the last dimension is contiguous" % what)
-    if rows is not None and t.shape[0] < rows:
-        raise ValueError("%s: %d rows, %d needed" % (what, t.shape[0], rows))
-    return t
+# A call of these is a few microseconds of work on the GPU, so the checks below
+# are written for few calls into torch each.
+
+def _on_gpu(what, first, *tensors):
+    """Every tensor (None = not given) is on `first`'s GPU."""
+    if not first.is_cuda:
+        raise ValueError("%s: a CUDA tensor, not one on %s" % (what, first.device))
+    device = first.get_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != device):
+            raise ValueError("%s: tensors on %s and %s" % (what, first.device, t.device))
+
+
+def _table(what, t, dtype, count):
+    """A contiguous tensor of `dtype` with at least `count` values."""
+    if t.dtype is not dtype or t.numel() < count or not t.is_contiguous():
+        raise ValueError("%s: %d contiguous values of %s, not %s of %s"
+                         % (what, count, dtype, tuple(t.shape), t.dtype))
 
 
 def _launch(fn, args, tensor, stream):
     """Calls `fn` on `tensor`'s device, whichever device is current."""
     import torch
-    if tensor.device.index == torch.cuda.current_device():
+    device = tensor.get_device()
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            N.check(fn(ctypes.byref(args), _stream_ptr(stream)))
+    elif stream is None:
+        N.check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)))
+    else:
         N.check(fn(ctypes.byref(args), _stream_ptr(stream)))
-        return
-    with torch.cuda.device(tensor.device):
-        N.check(fn(ctypes.byref(args), _stream_ptr(stream)))
-
-
-def _same_device(what, first, *others):
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError("%s: tensors on %s and %s" % (what, first.device, t.device))
 
 
 def pack_args(grids, *, offsets, image=None, positions=None, capacity=None, lead=0,
@@ -307,35 +311,37 @@ def pack_args(grids, *, offsets, image=None, positions=None, capacity=None, lead
     f32 ``[capacity][3]`` or None. ``capacity`` defaults to the rows of
     ``image`` or ``positions``."""
     import torch
-    _check("pack: grids", grids, torch.int32)
-    if grids.dim() != 2 or grids.shape[1] != 3 or not grids.is_contiguous():
-        raise ValueError("pack: grids are contiguous [images][3], not %s" % (tuple(grids.shape),))
-    n = grids.shape[0]
-    _check("pack: offsets", offsets, torch.int32, n + 1)
+    _on_gpu("pack", grids, offsets, image, positions)
+    shape = grids.shape
+    if len(shape) != 2 or shape[1] != 3:
+        raise ValueError("pack: grids are [images][3], not %s" % (tuple(shape),))
+    n = shape[0]
+    _table("pack: grids", grids, torch.int32, 3 * n)
+    _table("pack: offsets", offsets, torch.int32, n + 1)
     if capacity is None:
-        have = image if image is not None else positions
-        if have is None:
+        if image is None and positions is None:
             raise ValueError("pack: a capacity, an image map or positions")
-        capacity = have.shape[0]
+        capacity = (image if image is not None else positions).shape[0]
     if image is not None:
-        _check("pack: image", image, torch.int32, capacity)
+        _table("pack: image", image, torch.int32, capacity)
     if positions is not None:
-        _check("pack: positions", positions, torch.float32, capacity)
-        if positions.dim() != 2 or positions.shape[1] != 3 or not positions.is_contiguous():
-            raise ValueError("pack: positions are contiguous [capacity][3]")
+        _table("pack: positions", positions, torch.float32, 3 * capacity)
+        if positions.dim() != 2 or positions.shape[1] != 3:
+            raise ValueError("pack: positions are [capacity][3], not %s" % (tuple(positions.shape),))
     if not 0 <= lead < 2 ** 31 or not 0 <= capacity < 2 ** 31:
         raise ValueError("pack: %d lead rows, %d rows" % (lead, capacity))
-    _same_device("pack", grids, offsets, image, positions)
-    return N.PackArgs(images=n, capacity=capacity, lead=lead, normalized=1 if normalized else 0,
-                      grids=grids.data_ptr(), offsets=offsets.data_ptr(), image=_ptr(image),
-                      positions=_ptr(positions))
+    return N.PackArgs(n, capacity, lead, 1 if normalized else 0, grids.data_ptr(),
+                      offsets.data_ptr(), None if image is None else image.data_ptr(),
+                      None if positions is None else positions.data_ptr())
 
 
-def pack(grids, *, offsets, stream=None, **kw):
+def pack(grids, *, offsets, image=None, positions=None, capacity=None, lead=0, normalized=False,
+         stream=None):
     """Row maps of a packed batch, built on the GPU (``bl_pack``): each image's
     first row, each row's image and its patch's (t, y, x). Returns
     ``offsets``."""
-    a = pack_args(grids, offsets=offsets, **kw)
+    a = pack_args(grids, offsets=offsets, image=image, positions=positions, capacity=capacity,
+                  lead=lead, normalized=normalized)
     _launch(N.lib().bl_pack, a, grids, stream)
     return offsets
 
@@ -348,58 +354,66 @@ def rope_args(x, positions, *, sections, theta=100.0, freqs=None, shared=False, 
     more]``, the axes its first columns. ``sections``: the pairs of each axis.
     ``freqs``: the host's own radians a unit of position, one a pair."""
     import torch
-    _check("rope: x", x)
-    _check("rope: positions", positions, torch.float32)
-    out = x if out is None else _check("rope: out", out)
-    if x.dim() == 3:
-        if (heads or x.shape[1]) != x.shape[1] or (head_dim or x.shape[2]) != x.shape[2]:
-            raise ValueError("rope: %s heads of %s in %s" % (heads, head_dim, tuple(x.shape)))
-        heads, head_dim = x.shape[1], x.shape[2]
-    if x.dim() not in (2, 3) or not heads or not head_dim:
+    out = x if out is None else out
+    _on_gpu("rope", x, positions, out)
+    shape, axes = x.shape, len(sections)
+    rows = shape[0] if shape else 0
+    if len(shape) == 3:
+        if (heads or shape[1]) != shape[1] or (head_dim or shape[2]) != shape[2]:
+            raise ValueError("rope: %s heads of %s in %s" % (heads, head_dim, tuple(shape)))
+        heads, head_dim = shape[1], shape[2]
+    if len(shape) not in (2, 3) or not heads or not head_dim:
         raise ValueError("rope: x is [rows][heads][head_dim], or [rows][width] with both given")
-    rows = x.shape[0]
-    for what, t in (("x", x), ("out", out)):
-        if t.dim() == 3 and t.shape[1] > 1 and t.stride(1) != head_dim:
-            raise ValueError("rope: the heads of a row of %s are neighbours" % what)
-        if t.shape[0] != rows or (t.dim() == 3 and t.shape != x.shape) or \
-                t[0:1].numel() < heads * head_dim or t.dtype != x.dtype:
-            raise ValueError("rope: %s is %s of %s" % (what, tuple(t.shape), t.dtype))
-    axes = len(sections)
-    if not 1 <= axes <= 3 or positions.dim() != 2 or positions.shape[0] < rows or \
-            positions.shape[1] < axes:
-        raise ValueError("rope: positions %s for %d rows and %d axes (1 to 3)"
-                         % (tuple(positions.shape), rows, axes))
-    if any(int(n) < 1 for n in sections):
+    strides = []
+    for t in (x,) if out is x else (x, out):
+        have, st = t.shape, t.stride()
+        if t.dtype is not x.dtype or len(have) not in (2, 3) or have[0] != rows or \
+                (len(have) == 3 and tuple(have[1:]) != (heads, head_dim)) or \
+                (len(have) == 2 and have[1] < heads * head_dim):
+            raise ValueError("rope: %s of %s for %d rows of %d heads of %d"
+                             % (tuple(have), t.dtype, rows, heads, head_dim))
+        if rows and (st[-1] != 1 and head_dim > 1
+                     or len(have) == 3 and heads > 1 and st[1] != head_dim):
+            raise ValueError("rope: the values of a row's heads are neighbours")
+        strides.append(st[0] if rows > 1 else 0)
+    p_shape, p_stride = positions.shape, positions.stride()
+    if not 1 <= axes <= 3 or positions.dtype is not torch.float32 or len(p_shape) != 2 or \
+            p_shape[0] < rows or p_shape[1] < axes or (axes > 1 and p_stride[1] != 1):
+        raise ValueError("rope: positions %s of %s for %d rows and %d axes (1 to 3)"
+                         % (tuple(p_shape), positions.dtype, rows, axes))
+    if min(sections) < 1:
         raise ValueError("rope: sections %s" % (tuple(sections),))
-    if dtype is None and not x.dtype.is_floating_point:
-        raise ValueError("rope: the dtype of a %s container" % x.dtype)
-    if dtype is not None and (x.element_size() != (4 if dtype == "f32" else 2) or (
-            x.dtype.is_floating_point and _dt(x) != _TD[dtype])):
-        raise ValueError("rope: %s values in a tensor of %s" % (dtype, x.dtype))
-    _same_device("rope", x, positions, out)
-    a = N.RopeArgs(rows=rows, heads=heads, head_dim=head_dim, axes=axes, pairing=PAIRING[pairing],
-                   shared_ladder=1 if shared else 0, inverse=1 if inverse else 0,
-                   dtype=_dt(x) if dtype is None else _TD[dtype], theta=theta, x=x.data_ptr(),
-                   x_row_stride=x.stride(0) if rows > 1 else 0, positions=positions.data_ptr(),
-                   pos_row_stride=positions.stride(0) if rows > 1 else 0, out=out.data_ptr(),
-                   out_row_stride=out.stride(0) if rows > 1 else 0)
-    a.sections[:axes] = [int(n) for n in sections]
+    if dtype is None:
+        if not x.dtype.is_floating_point:
+            raise ValueError("rope: the dtype of a %s container" % x.dtype)
+        code = _dt(x)
+    else:
+        code = _TD[dtype]
+        if x.element_size() != (4 if dtype == "f32" else 2) or (
+                x.dtype.is_floating_point and _dt(x) != code):
+            raise ValueError("rope: %s values in a tensor of %s" % (dtype, x.dtype))
+    a = N.RopeArgs(rows, heads, head_dim, axes, tuple(sections), PAIRING[pairing],
+                   1 if shared else 0, 1 if inverse else 0, code, theta, None, x.data_ptr(),
+                   strides[0], positions.data_ptr(), p_stride[0] if rows > 1 else 0,
+                   out.data_ptr(), strides[-1])
     if freqs is not None:
-        if len(freqs) != sum(int(n) for n in sections):
+        if len(freqs) != sum(sections):
             raise ValueError("rope: %d frequencies for sections %s" % (len(freqs), tuple(sections)))
         a._freqs = (ctypes.c_double * len(freqs))(*[float(f) for f in freqs])
         a.freqs = ctypes.addressof(a._freqs)
     return a
 
 
-def rope(x, positions, *, sections, out=None, stream=None, **kw):
+def rope(x, positions, *, sections, theta=100.0, freqs=None, shared=False, pairing="half",
+         inverse=False, heads=None, head_dim=None, dtype=None, out=None, stream=None):
     """Rotary positions with 1 to 3 axes (``bl_rope``) on the heads of ``x``,
     in place or into ``out``; ``inverse=True`` turns back (the gradient)."""
-    out = x if out is None else out
-    a = rope_args(x, positions, sections=sections, out=out, **kw)
+    a = rope_args(x, positions, sections=sections, theta=theta, freqs=freqs, shared=shared,
+                  pairing=pairing, inverse=inverse, heads=heads, head_dim=head_dim, dtype=dtype,
+                  out=out)
     if a.rows:
         _launch(N.lib().bl_rope, a, x, stream)
-    return out
+    return x if out is None else out
 
 
 def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets=None,
@@ -414,27 +428,27 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
     int32 ``[batch]``; ``slopes``: f32 ``[heads]``; ``positions``: f32
     ``[rows][1 to 3 axes]``."""
     import torch
-    if head_rows := (qkv.dim() == 3):
-        if qkv.shape[2] != 64 or (qkv.shape[1] > 1 and qkv.stride(1) != 64):
-            raise ValueError("masked attention: qkv rows of neighbouring heads of 64, not %s"
-                             % (tuple(qkv.shape),))
-    _check("masked attention: qkv", qkv)
-    _check("masked attention: out", out)
+    _on_gpu("masked attention", qkv, out, offsets, lengths, prefix, slopes, positions)
     kv = heads if kv_heads is None else kv_heads
-    rows, width = qkv.shape[0], qkv.shape[1] * (64 if head_rows else 1)
-    if qkv.element_size() != 2 or qkv.dim() not in (2, 3) or heads < 1 or kv < 1 or \
+    shape, st = qkv.shape, qkv.stride()
+    if len(shape) == 3:
+        ok = shape[2] == 64 and (shape[1] <= 1 or st[1] == 64)
+        width = shape[1] * 64
+    else:
+        ok, width = len(shape) == 2, shape[-1] if shape else 0
+    if not ok or st[-1] != 1 or qkv.element_size() != 2 or heads < 1 or kv < 1 or \
             width < (heads + 2 * kv) * 64:
-        raise ValueError("masked attention: qkv is %s of %s for %d heads and %d K/V heads"
-                         % (tuple(qkv.shape), qkv.dtype, heads, kv))
-    if out.dim() != 2 or out.shape[0] < rows or out.shape[1] < heads * 64:
-        raise ValueError("masked attention: out is %s for %d rows" % (tuple(out.shape), rows))
+        raise ValueError("masked attention: qkv is %s (strides %s) of %s for %d heads and %d K/V "
+                         "heads of 64 side by side" % (tuple(shape), st, qkv.dtype, heads, kv))
+    rows = shape[0]
+    o_shape, o_st = out.shape, out.stride()
+    if len(o_shape) != 2 or o_shape[0] < rows or o_shape[1] < heads * 64 or o_st[1] != 1:
+        raise ValueError("masked attention: out is %s for %d rows of %d" % (tuple(o_shape), rows,
+                                                                          heads * 64))
     if offsets is not None:
-        _check("masked attention: offsets", offsets, torch.int32)
         if batch is None:
             batch = offsets.numel() - 1
-        if offsets.numel() < batch + 1 or not offsets.is_contiguous():
-            raise ValueError("masked attention: %d offsets for %d sequences"
-                             % (offsets.numel(), batch))
+        _table("masked attention: offsets", offsets, torch.int32, batch + 1)
         tokens = rows
     else:
         if batch is None:
@@ -442,31 +456,32 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
         if batch < 1 or rows % batch:
             raise ValueError("masked attention: %d rows in %d equal parts" % (rows, batch))
         tokens = rows // batch
-    for what, t, n, dt in (("lengths", lengths, batch, torch.int32),
-                           ("prefix", prefix, batch, torch.int32),
-                           ("slopes", slopes, heads, torch.float32)):
-        if t is not None and (_check("masked attention: " + what, t, dt).numel() < n
-                              or not t.is_contiguous()):
-            raise ValueError("masked attention: %d %s, %d needed" % (t.numel(), what, n))
+    if lengths is not None:
+        _table("masked attention: lengths", lengths, torch.int32, batch)
+    if prefix is not None:
+        _table("masked attention: prefix", prefix, torch.int32, batch)
+    if slopes is not None:
+        _table("masked attention: slopes", slopes, torch.float32, heads)
+    axes = pos_stride = 0
     if positions is not None:
-        _check("masked attention: positions", positions, torch.float32, rows)
-        if positions.dim() != 2 or not 1 <= positions.shape[1] <= 3:
-            raise ValueError("masked attention: positions are [rows][1 to 3], not %s"
-                             % (tuple(positions.shape),))
+        p_shape, p_st = positions.shape, positions.stride()
+        if positions.dtype is not torch.float32 or len(p_shape) != 2 or p_shape[0] < rows or \
+                not 1 <= p_shape[1] <= 3 or (p_shape[1] > 1 and p_st[1] != 1):
+            raise ValueError("masked attention: positions are f32 [rows][1 to 3], not %s of %s"
+                             % (tuple(p_shape), positions.dtype))
+        axes, pos_stride = p_shape[1], p_st[0] if rows > 1 else 0
     if last_rows < 0 or (cap is not None and not cap > 0):
         raise ValueError("masked attention: last_rows %s, cap %s" % (last_rows, cap))
-    _same_device("masked attention", qkv, out, offsets, lengths, prefix, slopes, positions)
     many = rows > 1
     return N.MaskedAttentionArgs(
-        batch=batch, tokens=tokens, heads=heads, kv_heads=kv, head_dim=64,
-        last_rows=min(last_rows, 2 ** 31 - 1), scale=0.125 if scale is None else scale,
-        cap=0.0 if cap is None else cap, mask=MASK[mask], qk_dtype=_TD[qk_dtype],
-        v_dtype=N.BL_F16, out_dtype=_dt(out) if out_dtype is None else _TD[out_dtype],
-        qkv=qkv.data_ptr(), qkv_row_stride=qkv.stride(0) if many else 0, out=out.data_ptr(),
-        out_row_stride=out.stride(0) if many else 0, offsets=_ptr(offsets), lengths=_ptr(lengths),
-        prefix=_ptr(prefix), slopes=_ptr(slopes), positions=_ptr(positions),
-        pos_row_stride=positions.stride(0) if positions is not None and many else 0,
-        pos_axes=0 if positions is None else positions.shape[1], key_splits=key_splits)
+        batch, tokens, heads, kv, 64, min(last_rows, 2 ** 31 - 1),
+        0.125 if scale is None else scale, cap or 0.0, MASK[mask], _TD[qk_dtype], N.BL_F16,
+        _dt(out) if out_dtype is None else _TD[out_dtype], qkv.data_ptr(), st[0] if many else 0,
+        out.data_ptr(), o_st[0] if many else 0, None if offsets is None else offsets.data_ptr(),
+        None if lengths is None else lengths.data_ptr(),
+        None if prefix is None else prefix.data_ptr(),
+        None if slopes is None else slopes.data_ptr(),
+        None if positions is None else positions.data_ptr(), pos_stride, axes, key_splits)
 
 
 def masked_attention(qkv, *, heads, out=None, out_dtype=None, stream=None, **kw):
@@ -474,12 +489,15 @@ def masked_attention(qkv, *, heads, out=None, out_dtype=None, stream=None, **kw)
     distance and document, causal or prefix masks (``bl_masked_attention``);
     ``last_rows`` computes the newest rows of every sequence alone. Without
     ``out`` a zero-filled ``[rows][heads * 64]`` of ``out_dtype`` (default
-    "f16") is made; rows that are not computed are left as they were."""
+    "f16") is made on the stream; rows that are not computed are left as they
+    were."""
     import torch
     if out is None:
         tdt = {"f32": torch.float32, "f16": torch.float16,
                "bf16": torch.bfloat16}[out_dtype or "f16"]
-        out = torch.zeros((qkv.shape[0], heads * 64), dtype=tdt, device=qkv.device)
+        s = torch.cuda.ExternalStream(stream, device=qkv.device) if isinstance(stream, int) else stream
+        with torch.cuda.stream(s):  # (None: the current one)
+            out = torch.zeros((qkv.shape[0], heads * 64), dtype=tdt, device=qkv.device)
         out_dtype = None
     elif out.dtype.is_floating_point:
         if out_dtype is not None and _dt(out) != _TD[out_dtype]:
