@@ -444,18 +444,38 @@ struct TileTail {
     int t0, n;      // its key tiles
     float ref[2][BM];      // R after the stream's last tile
     float odd_sum[BM];
-    float kpos[8][3][BN];  // each softmax warp's copy of a key tile's positions
+    alignas(16) float kpos[8][3][BN];  // each softmax warp's copy of a key tile's positions
 };
 constexpr size_t kTileSmem = 1024 + kQBytes + 2 * STAGES * kKvBytes + sizeof(TileTail);
 static_assert(2 * (kTileSmem + 1024) <= 233472, "two CTAs an SM");
 
 // The sequence (its rows, without the prefix) and tile of tile `index` of the
-// packed batch: a warp walks the offsets 256 sequences at a time, eight a lane,
-// so a chunk costs one round trip to memory. Returns the sequence, -1 behind
-// the last tile.
+// packed batch, the longest sequences' tiles first while there are at most 32
+// (a warp ranks them by their lengths); otherwise in the sequences' order, which
+// a warp walks 256 at a time, eight a lane, so that a chunk costs one round trip
+// to memory. Returns the sequence, -1 behind the last tile.
 __device__ __forceinline__ int find_tile(const Params& p, int index, int& begin, int& len,
                                          int& tile) {
     const int lane = lane_id();
+    if (p.batch <= 32) {
+        // one sequence a lane: the tiles of the longer ones come before its own
+        const int b = min(max(p.offsets[min(lane, p.batch)], 0), p.tokens);
+        const int e = min(max(p.offsets[min(lane + 1, p.batch)], 0), p.tokens);
+        const int rows = max(e - b, 0);
+        int before = 0;
+        for (int j = 0; j < p.batch; ++j) {
+            const int other = __shfl_sync(0xFFFFFFFFu, rows, j);
+            if (other > rows || (other == rows && j < lane)) before += (other + BM - 1) / BM;
+        }
+        const bool here = index >= before && index < before + (rows + BM - 1) / BM;
+        const unsigned found = __ballot_sync(0xFFFFFFFFu, here);
+        if (found == 0) return -1;
+        const int owner = __ffs(found) - 1;
+        begin = __shfl_sync(0xFFFFFFFFu, b, owner);
+        len = __shfl_sync(0xFFFFFFFFu, rows, owner);
+        tile = __shfl_sync(0xFFFFFFFFu, index - before, owner);
+        return owner;
+    }
     int total = 0;
     for (int base = 0; base < p.batch; base += 256) {
         const int first = base + 8 * lane;
@@ -524,6 +544,36 @@ __device__ __forceinline__ void store8(void* out, long long at, int dt, const fl
     }
 }
 
+// cap tanh(s / cap) of two raw scores in log2 units. Where every |u| = |s / cap|
+// of the warp's tile is at most kSmallTanh, by the odd series through u^9 on
+// the FMA units (the first term left out is below 10^-6 of the value there),
+// which spares the unit that the exponentials need two of its three functions
+// a score; otherwise by those.
+constexpr float kSmallTanh = 0.4f;
+struct Capping {
+    float unit;   // raw score -> u
+    float scale;  // raw score -> log2 units, uncapped
+    float twice;  // raw score -> 2 u in log2 units
+    float cap2;   // cap in log2 units
+};
+__device__ __forceinline__ unsigned long long both(float v) { return f2pack(v, v); }
+__device__ __forceinline__ unsigned long long capped2(unsigned long long s, const Capping& k,
+                                                      bool small) {
+    if (small) {
+        const unsigned long long u = fmul2(s, both(k.unit)), v = fmul2(u, u);
+        unsigned long long c = ffma2(v, both(62.0f / 2835.0f), both(-17.0f / 315.0f));
+        c = ffma2(v, c, both(2.0f / 15.0f));
+        c = ffma2(v, c, both(-1.0f / 3.0f));
+        const unsigned long long w = fmul2(s, both(k.scale));
+        return ffma2(fmul2(w, v), c, w);
+    }
+    float a, b;
+    f2unpack(s, a, b);
+    a = fmaf(rcp_approx(1.0f + ex2(a * k.twice)), -2.0f * k.cap2, k.cap2);
+    b = fmaf(rcp_approx(1.0f + ex2(b * k.twice)), -2.0f * k.cap2, k.cap2);
+    return f2pack(a, b);
+}
+
 enum { BIAS_NONE = 0, BIAS_INDEX = 1, BIAS_PLANE = 2, BIAS_SPACE = 3 };
 
 template <bool kCap, int kBias>
@@ -539,7 +589,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     TileTail* tail = reinterpret_cast<TileTail*>(sV + STAGES * kKvBytes);
     volatile int* abort = &tail->abort;
     const int warp = warp_id(), lane = lane_id();
-    const int head = blockIdx.y, kvh = head / p.group;
+    // CTAs in the order of their start: the splits of a unit side by side (a
+    // cluster), then the heads of a tile, so that the tiles with most keys (the
+    // first units) start first in every head and the last CTAs are short
+    const unsigned work = blockIdx.x / static_cast<unsigned>(p.splits);
+    const unsigned split = blockIdx.x - work * p.splits;
+    const int unit = static_cast<int>(work / static_cast<unsigned>(p.heads));
+    const int head = static_cast<int>(work - static_cast<unsigned>(unit) * p.heads);
+    const int kvh = head / p.group;
     constexpr unsigned kFull = 0xFFFFFFFFu;
 
     if (threadIdx.x == 0) {
@@ -571,13 +628,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     pdl_wait();
     if (warp == 0) {
         __syncwarp();
-        const int unit = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.splits));
-        const unsigned split = blockIdx.x - static_cast<unsigned>(unit) * p.splits;
         Span q{};
         int tile = 0, rows = 0, q0 = 0, first = 0, count = 0;
         if (p.chunks > 0) {
-            q = span_of(p, unit / p.chunks);
-            tile = unit % p.chunks;
+            q = span_of(p, unit % p.batch);
+            tile = unit / p.batch;
         } else {
             int begin = 0;
             const int seq = find_tile(p, unit, begin, q.len, tile);
@@ -587,8 +642,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
         const int tiles = (q.len - q.first + BM - 1) / BM;
         if (tile >= 0 && tile < tiles) {
-            // with a causal mask the last rows see most: they start first
-            if (p.mask != BL_MASK_NONE) tile = tiles - 1 - tile;
+            tile = tiles - 1 - tile;  // with a causal mask the last rows see most
             q0 = q.first + tile * BM;
             rows = min(q.len - q0, BM);
             // below 2^25 tiles and at most 8 splits: 32 bits hold the products
@@ -744,11 +798,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         const bool live = row < tail->rows;
         const int seen = live ? visible(p, q, at) : 0;
         constexpr bool kPlain = !kCap && kBias == BIAS_NONE;
-        // kPlain keeps raw scores and scales them in the exponent's FMA; the
-        // other forms turn each score into log2 units first
-        const float c = kPlain ? p.scale * kLog2e : 1.0f;
-        const float in = kCap ? 2.0f * p.scale / p.cap * kLog2e : p.scale * kLog2e;
-        const float cap2 = p.cap * kLog2e;
+        constexpr bool kCapOnly = kCap && kBias == BIAS_NONE;
+        // raw scores to log2 units; kPlain does it in the exponent's FMA
+        const float in = p.scale * kLog2e;
+        const Capping cap{kCap ? p.scale / p.cap : 0.0f, in, kCap ? 2.0f * p.scale / p.cap * kLog2e : 0.0f,
+                          p.cap * kLog2e};
         const float slope2 = kBias != BIAS_NONE ? p.slopes[head] * kLog2e : 0.0f;
         float qp[3] = {0.0f, 0.0f, 0.0f};
         if (kBias >= BIAS_PLANE) {
@@ -761,21 +815,31 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         bool ok = true;
         // tile i: S buffer `buf` = i % SBUFS, whose use it is the phase of
         int buf = odd, phase = 0;
+        // the positions of this lane's two keys of the next tile
+        constexpr int kAxes = kBias == BIAS_SPACE ? 3 : 2;
+        float ahead[kAxes][2];
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int a = 0; a < kAxes; ++a)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = (t0 + i) * BN + lane + 32 * e;
+                    ahead[a][e] = i < n && key < q.len && a < p.pos_axes
+                                      ? p.pos[(q.begin + key) * p.pos_row + a] : 0.0f;
+                }
+        };
+        if (kBias >= BIAS_PLANE) fetch(odd);
         for (int i = odd; i < n; i += 2) {
             const int k0 = (t0 + i) * BN;
             if (kBias >= BIAS_PLANE) {
                 __syncwarp();  // every lane is done with the last tile's copy
-                constexpr int kAxes = kBias == BIAS_SPACE ? 3 : 2;
 #pragma unroll
                 for (int a = 0; a < kAxes; ++a)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int key = k0 + lane + 32 * e;
-                        tail->kpos[warp - kSoftmaxWarp0][a][lane + 32 * e] =
-                            key < q.len && a < p.pos_axes ? p.pos[(q.begin + key) * p.pos_row + a]
-                                                          : 0.0f;
-                    }
+                    for (int e = 0; e < 2; ++e)
+                        tail->kpos[warp - kSoftmaxWarp0][a][lane + 32 * e] = ahead[a][e];
                 __syncwarp();
+                fetch(i + 2);
             }
             const uint32_t s_col = t_lane + BN * buf;
             ok = wait_warp(&tail->s_full[buf], phase, ST_TIMEOUT_SOFTMAX, i);
@@ -785,30 +849,77 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             // some row of the warp sees less than the whole tile
             const bool cut = __any_sync(kFull, valid < BN);
             const float rel = static_cast<float>(at - k0);
+            // |i - j| is linear over the tile where all its keys lie on one
+            // side of all the warp's rows: the bias of key k is then
+            // lean (k - rel), and takes part in the scaling's FMA
+            const int row0 = tail->q0 + sub * 32;
+            const bool before = k0 + BN - 1 <= row0, after = k0 >= row0 + 31;
+            const bool linear = kBias == BIAS_INDEX && !kCap && (before || after);
+            const float lean = before ? slope2 : -slope2;
+            // the biases of keys k and k + 1, formed anew every eighth key
+            auto lean2 = [&](int k, float less) {
+                const float b = fmaf(lean, static_cast<float>(k) - rel, -less);
+                return f2pack(b, b + lean);
+            };
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float far = 0.0f;  // the largest |score|, for the capping's choice
+            bool small = false;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t s[32];
                 tmem_ld32(s_col + 32 * h, s);
                 tmem_wait_ld();
-                if (!kPlain) {
+                auto pair = [&](int e) {
+                    return f2pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+                };
+                auto set = [&](int e, unsigned long long v) {
+                    float x, y;
+                    f2unpack(v, x, y);
+                    s[2 * e] = __float_as_uint(x), s[2 * e + 1] = __float_as_uint(y);
+                };
+                if (kCap) {
+                    float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int k = 32 * h + e;
-                        float t = __uint_as_float(s[e]) * in;
-                        if (kCap) t = fmaf(rcp_approx(1.0f + ex2(t)), -2.0f * cap2, cap2);
-                        if (kBias == BIAS_INDEX)
-                            t = fmaf(-slope2, fabsf(rel - static_cast<float>(k)), t);
-                        if (kBias >= BIAS_PLANE) {
-                            const float x = qp[0] - kpos[0][k], y = qp[1] - kpos[1][k];
-                            float d2 = fmaf(x, x, y * y);
-                            if (kBias == BIAS_SPACE) {
-                                const float z = qp[2] - kpos[2][k];
-                                d2 = fmaf(z, z, d2);
+                    for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            f[j] = fmax3(f[j], fabsf(__uint_as_float(s[e + 2 * j])),
+                                         fabsf(__uint_as_float(s[e + 2 * j + 1])));
+                    far = fmax3(fmaxf(far, f[0]), fmaxf(f[1], f[2]), f[3]);
+                    small = !__any_sync(kFull, far * cap.unit > kSmallTanh);
+                }
+                if (linear) {
+                    unsigned long long b = 0;
+                    const unsigned long long step = both(2.0f * lean), in2 = both(in);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        b = e % 4 == 0 ? lean2(32 * h + 2 * e, 0.0f) : fadd2(b, step);
+                        set(e, ffma2(pair(e), in2, b));
+                    }
+                } else if (kBias != BIAS_NONE) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int k = 32 * h + 2 * e;
+                        unsigned long long t = kCap ? capped2(pair(e), cap, small)
+                                                    : fmul2(pair(e), both(in));
+                        unsigned long long d;
+                        if (kBias == BIAS_INDEX) {
+                            d = f2pack(fabsf(rel - static_cast<float>(k)),
+                                       fabsf(rel - static_cast<float>(k + 1)));
+                        } else {
+                            // the distance from each key's copy of its place
+                            unsigned long long d2 = 0;
+#pragma unroll
+                            for (int a = 0; a < (kBias == BIAS_SPACE ? 3 : 2); ++a) {
+                                const float2 w = *reinterpret_cast<const float2*>(&kpos[a][k]);
+                                const unsigned long long x = fadd2(both(qp[a]), f2pack(-w.x, -w.y));
+                                d2 = a == 0 ? fmul2(x, x) : ffma2(x, x, d2);
                             }
-                            t = fmaf(-slope2, sqrt_approx(d2), t);
+                            float x, y;
+                            f2unpack(d2, x, y);
+                            d = f2pack(sqrt_approx(x), sqrt_approx(y));
                         }
-                        s[e] = __float_as_uint(t);
+                        set(e, ffma2(both(-slope2), d, t));
                     }
                 }
                 if (cut) {
@@ -822,10 +933,15 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                     for (int j = 0; j < 4; ++j)
                         mx[j] = fmax3(mx[j], __uint_as_float(s[e + 2 * j]),
                                       __uint_as_float(s[e + 2 * j + 1]));
-                if (!kPlain) tmem_st32(s_col + 32 * h, s);
+                if (kBias != BIAS_NONE && !linear) tmem_st32(s_col + 32 * h, s);
             }
-            if (!kPlain) tmem_wait_st();
-            const float m_row = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+            if (kBias != BIAS_NONE && !linear) tmem_wait_st();
+            float m_row = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+            if (kPlain) m_row *= in;
+            // (capping keeps the order: the largest capped score is the capped
+            // largest)
+            if (kCapOnly && m_row != -INFINITY)
+                m_row = fmaf(rcp_approx(1.0f + ex2(m_row * cap.twice)), -2.0f * cap.cap2, cap.cap2);
             // R(i) from R(i - 1), the other stream's, and this tile's maximum
             float prev = -INFINITY;
             if (i > 0) {
@@ -834,7 +950,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 if (!ok) break;
                 prev = tail->ref[odd ^ 1][row];
             }
-            const float m_new = fmaxf(prev, m_row * c);
+            const float m_new = fmaxf(prev, m_row);
             const bool need = m_new > prev + kRescaleThreshold;
             const float now = need ? m_new : prev;
             tail->ref[odd][row] = now;
@@ -865,26 +981,52 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             // a row that has seen no key yet (another split's, or none) has no
             // maximum: its exponents are taken against 0
             const float nm = m_used == -INFINITY ? 0.0f : -m_used;
-            const unsigned long long nm2 = f2pack(nm, nm), c2 = f2pack(c, c);
-            unsigned long long acc[2] = {f2pack(0.0f, 0.0f), f2pack(0.0f, 0.0f)};
+            const unsigned long long nm2 = both(nm);
+            unsigned long long acc[2] = {both(0.0f), both(0.0f)};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t s[32];
                 tmem_ld32(s_col + 32 * h, s);
                 tmem_wait_ld();
-                if (kPlain && cut) {
+                if (kCapOnly) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float x, y;
+                        f2unpack(capped2(f2pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])),
+                                         cap, small), x, y);
+                        s[2 * e] = __float_as_uint(x), s[2 * e + 1] = __float_as_uint(y);
+                    }
+                }
+                // (scores stored back in the first pass are masked already)
+                if ((kPlain || kCapOnly || linear) && cut) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (32 * h + e >= valid) s[e] = __float_as_uint(-INFINITY);
                 }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                auto finish = [&](int e, unsigned long long x) {
                     float x0, x1;
-                    f2unpack(ffma2(f2pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])),
-                                   c2, nm2), x0, x1);
+                    f2unpack(x, x0, x1);
                     x0 = ex2(x0), x1 = ex2(x1);
                     acc[e & 1] = fadd2(acc[e & 1], f2pack(x0, x1));
                     s[e] = pack_f16x2(x0, x1);
+                };
+                auto pair = [&](int e) {
+                    return f2pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+                };
+                if (kPlain) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) finish(e, ffma2(pair(e), both(in), nm2));
+                } else if (kBias == BIAS_INDEX && linear) {
+                    const unsigned long long in2 = both(in), step = both(2.0f * lean);
+                    unsigned long long b = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        b = e % 4 == 0 ? lean2(32 * h + 2 * e, -nm) : fadd2(b, step);
+                        finish(e, ffma2(pair(e), in2, b));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) finish(e, fadd2(pair(e), nm2));
                 }
                 // P's columns [16 h, 16 h + 16) lie over scores already read
                 tmem_st16(s_col + 16 * h, s);
@@ -1118,7 +1260,7 @@ int prepare_tiles(const bl_masked_attention_args& a, Launch* out) {
     p.splits = a.key_splits ? static_cast<int>(a.key_splits)
                             : static_cast<int>(std::max<uint64_t>(
                                   1, std::min<uint64_t>({8, 296 / (units * p.heads), keys / 256})));
-    if (units * p.splits > 0x7FFFFFFFull)
+    if (units * p.heads * p.splits > 0x7FFFFFFFull)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: grid too large");
     const uint64_t rows = a.offsets != nullptr ? a.tokens : 1ull * a.batch * a.tokens;
     CUtensorMap tm_q, tm_kv;
@@ -1141,7 +1283,7 @@ int prepare_tiles(const bl_masked_attention_args& a, Launch* out) {
     const Kern kern = kerns[p.cap > 0.0f ? 1 : 0][bias];
     BL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      static_cast<int>(kTileSmem)));
-    const dim3 grid(static_cast<unsigned>(units * p.splits), p.heads);
+    const dim3 grid(static_cast<unsigned>(units * p.heads * p.splits));
     const int bf16 = a.qk_dtype == BL_BF16;
     out->op = BL_OP_MASKED_ATTENTION;
     out->run = [=](cudaStream_t s) {

@@ -6,7 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
-#include <new>
+#include <type_traits>
 
 #include "host.h"
 
@@ -58,37 +58,154 @@ __global__ void __launch_bounds__(1024) pack_offsets_kernel(const int* grids, in
     if (threadIdx.x == 0 && total > cap) record_status(status, ST_BAD_ARGS, 0x9A);
 }
 
-// Image and position of each row: a binary search of the offsets (the last
-// image that starts at or before the row, so images without rows are passed
-// over), then the patch's (t, y, x).
-__global__ void __launch_bounds__(256) pack_rows_kernel(const int* grids, const int* offsets,
-                                                        int images, int lead, int normalized,
-                                                        long long cap, int* image, float* pos) {
-    pdl_trigger();
-    pdl_wait();
-    const long long r = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    if (r >= cap) return;
+// The last image that starts at or before row r (so images without rows are
+// passed over): `images` behind the last.
+__device__ __forceinline__ int image_of(const int* offsets, int images, int r) {
     int lo = 0, hi = images;  // offsets[lo] <= r
     while (lo < hi) {
         const int mid = lo + (hi - lo + 1) / 2;
         if (offsets[mid] <= r) lo = mid; else hi = mid - 1;
     }
-    const bool real = lo < images;
-    if (image != nullptr) image[r] = real ? lo : -1;
-    if (pos == nullptr) return;
-    float c[3] = {0.0f, 0.0f, 0.0f};
-    const long long p = real ? r - offsets[lo] - lead : -1;
-    if (p >= 0) {
-        const int* g = grids + 3ll * lo;
-        const unsigned u = static_cast<unsigned>(p), h = g[1], w = g[2];
-        const unsigned row = u / w, at[3] = {row / h, row % h, u % w};
-        for (int a = 0; a < 3; ++a) {
-            const float n = static_cast<float>(g[a]);
-            c[a] = normalized ? static_cast<float>(2ll * at[a] + 1 - g[a]) / n
-                              : static_cast<float>(at[a]);
+    return lo;
+}
+
+// Rows 4 k .. 4 k + 3 for k = first, first + step, ..: their image is searched
+// once, the patch's place divided out once, and both stepped from row to row,
+// so that a thread's four positions leave as three 16-byte stores.
+__device__ __forceinline__ void write_rows(const int* grids, const int* offsets, int images,
+                                           int lead, bool normalized, int cap, int* image,
+                                           float* pos, bool vec, int first, int step) {
+    const int groups = cap / 4 + (cap % 4 != 0);
+    for (int k = first; k < groups; k += step) {
+        int r = 4 * k;
+        int at = image_of(offsets, images, r);
+        int end = at < images ? offsets[at + 1] : cap, p = 0, c[3] = {0, 0, 0}, g[3] = {1, 1, 1};
+        float size[3] = {1.0f, 1.0f, 1.0f}, inverse[3] = {1.0f, 1.0f, 1.0f};
+        auto enter = [&]() {  // row r's place in image `at`
+            p = r - offsets[at] - lead;
+            if (at < images)
+                for (int a = 0; a < 3; ++a) g[a] = grids[3ll * at + a];
+            if (normalized)
+#pragma unroll
+                for (int a = 0; a < 3; ++a)
+                    size[a] = static_cast<float>(g[a]), inverse[a] = 1.0f / size[a];
+            const unsigned u = p > 0 ? p : 0, w = g[2], h = g[1], row = u / w;
+            c[0] = row / h, c[1] = row % h, c[2] = u % w;
+        };
+        if (at < images) enter();
+        int im[4];
+        float out[12];
+#pragma unroll
+        for (int i = 0; i < 4; ++i, ++r) {
+            if (at < images && r >= end) {
+                at = image_of(offsets, images, r);
+                end = at < images ? offsets[at + 1] : cap;
+                if (at < images) enter();
+            }
+            const bool real = at < images;
+            im[i] = real ? at : -1;
+#pragma unroll
+            for (int a = 0; a < 3; ++a) {
+                float v = static_cast<float>(c[a]);
+                if (normalized) {
+                    // (2 c + 1 - n) / n: the correctly rounded quotient from
+                    // the correctly rounded reciprocal (Markstein's
+                    // correction step), one division an image and axis
+                    const float x = static_cast<float>(2ll * c[a] + 1 - g[a]);
+                    const float q = x * inverse[a];
+                    v = fmaf(fmaf(-q, size[a], x), inverse[a], q);
+                }
+                out[3 * i + a] = !real || p < 0 ? 0.0f : v;
+            }
+            if (++p > 0) {
+                if (++c[2] == g[2]) {
+                    c[2] = 0;
+                    if (++c[1] == g[1]) c[1] = 0, ++c[0];
+                }
+            }
+        }
+        if (vec && 4 * k + 4 <= cap) {
+            if (image != nullptr)
+                reinterpret_cast<int4*>(image)[k] = make_int4(im[0], im[1], im[2], im[3]);
+            if (pos != nullptr)
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    reinterpret_cast<float4*>(pos)[3ll * k + e] =
+                        make_float4(out[4 * e], out[4 * e + 1], out[4 * e + 2], out[4 * e + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (4 * k + i >= cap) break;
+                if (image != nullptr) image[4 * k + i] = im[i];
+                if (pos != nullptr)
+#pragma unroll
+                    for (int a = 0; a < 3; ++a) pos[3ll * (4 * k + i) + a] = out[3 * i + a];
+            }
         }
     }
-    for (int a = 0; a < 3; ++a) pos[3 * r + a] = c[a];
+}
+
+__global__ void __launch_bounds__(256) pack_rows_kernel(const int* grids, const int* offsets,
+                                                        int images, int lead, int normalized,
+                                                        int cap, int* image, float* pos, int vec) {
+    pdl_trigger();
+    pdl_wait();
+    write_rows(grids, offsets, images, lead, normalized != 0, cap, image, pos, vec != 0,
+               static_cast<int>(blockIdx.x) * 256 + threadIdx.x, gridDim.x * 256);
+}
+
+// All of it in one launch for up to kPackImages images: every block scans the
+// sizes into its own shared memory (12 KB of reads from L2 and one block scan,
+// cheaper than a second launch and its wait) and writes its rows; block 0
+// writes the offsets. MEASURED_PACK
+constexpr int kPackImages = 4096;
+constexpr int kPackEach = kPackImages / 256;  // images a thread scans at most
+__global__ void __launch_bounds__(256) pack_kernel(const int* grids, int images, int lead,
+                                                   int normalized, int cap, int* offsets,
+                                                   int* image, float* pos, int vec,
+                                                   Status* status) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ int at[kPackImages + 1];
+    __shared__ long long warp_sum[8];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int each = (images + 255) / 256;
+    long long mine = 0, before[kPackEach];
+#pragma unroll
+    for (int e = 0; e < kPackEach; ++e) {
+        before[e] = mine;
+        const int i = t * each + e;
+        if (e < each && i < images) mine += image_rows(grids + 3ll * i, lead, cap);
+    }
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        if (lane >= o) upto += u;
+    }
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    long long base = upto - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        if (w < warp) base += warp_sum[w];
+        total += warp_sum[w];
+    }
+#pragma unroll
+    for (int e = 0; e < kPackEach; ++e) {
+        const int i = t * each + e;
+        if (e < each && i < images)
+            at[i] = static_cast<int>(min(base + before[e], static_cast<long long>(cap)));
+    }
+    if (t == 0) at[images] = static_cast<int>(min(total, static_cast<long long>(cap)));
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int i = t; i <= images; i += 256) offsets[i] = at[i];
+        if (t == 0 && total > cap) record_status(status, ST_BAD_ARGS, 0x9A);
+    }
+    if (image != nullptr || pos != nullptr)
+        write_rows(grids, at, images, lead, normalized != 0, cap, image, pos, vec != 0,
+                   static_cast<int>(blockIdx.x) * 256 + t, gridDim.x * 256);
 }
 
 // ------------------------------------------------------------------ rotary
@@ -124,6 +241,56 @@ struct alignas(sizeof(T) * kVec) Vec {
     T v[kVec];
 };
 
+// Values 2 w and 2 w + 1 of a vector, and back: 16-bit types by the word.
+template <typename T, int kVec>
+__device__ __forceinline__ float2 get2(const Vec<T, kVec>& x, int w) {
+    if constexpr (sizeof(T) == 4) {
+        return make_float2(x.v[2 * w], x.v[2 * w + 1]);
+    } else {
+        const uint32_t word = reinterpret_cast<const uint32_t*>(&x)[w];
+        if constexpr (std::is_same<T, __nv_bfloat16>::value)
+            return make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xFFFF0000u));
+        else
+            return __half22float2(*reinterpret_cast<const __half2*>(&word));
+    }
+}
+template <typename T, int kVec>
+__device__ __forceinline__ void put2(Vec<T, kVec>& x, int w, float lo, float hi) {
+    if constexpr (sizeof(T) == 4) {
+        x.v[2 * w] = lo, x.v[2 * w + 1] = hi;
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        reinterpret_cast<uint32_t*>(&x)[w] = pack_bf16x2(lo, hi);
+    } else {
+        reinterpret_cast<uint32_t*>(&x)[w] = pack_f16x2(lo, hi);
+    }
+}
+// The kVec pairs that the vectors a and b of one head hold, turned in place.
+template <typename T, int kVec, bool kAdjacent>
+__device__ __forceinline__ void turn_pairs(Vec<T, kVec>& a, Vec<T, kVec>& b, const float (&c)[kVec],
+                                           const float (&s)[kVec]) {
+    if constexpr (kVec == 1) {
+        const float f = up(a.v[0]), g = up(b.v[0]);
+        a.v[0] = down<T>(f * c[0] - g * s[0]);
+        b.v[0] = down<T>(g * c[0] + f * s[0]);
+    } else if constexpr (kAdjacent) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            Vec<T, kVec>& x = 2 * e < kVec ? a : b;
+            const int w = e % (kVec / 2);
+            const float2 f = get2(x, w);
+            put2(x, w, f.x * c[e] - f.y * s[e], f.y * c[e] + f.x * s[e]);
+        }
+    } else {
+#pragma unroll
+        for (int w = 0; w < kVec / 2; ++w) {
+            const float2 f = get2(a, w), g = get2(b, w);
+            const float c0 = c[2 * w], c1 = c[2 * w + 1], s0 = s[2 * w], s1 = s[2 * w + 1];
+            put2(a, w, f.x * c0 - g.x * s0, f.y * c1 - g.y * s1);
+            put2(b, w, g.x * c0 + f.x * s0, g.y * c1 + f.y * s1);
+        }
+    }
+}
+
 // A block turns tiles of rows, each thread kVec neighbouring pairs of several
 // heads: two vectors of a head (its halves, an axis's halves, or neighbours),
 // so every global access is a whole vector and a warp's cover whole sectors.
@@ -135,7 +302,7 @@ struct alignas(sizeof(T) * kVec) Vec {
 // tables (so one barrier a tile is enough), while the tile's values are on
 // their way; a thread keeps the frequency of its pair over all its tiles.
 // 60280 rows x 32 heads x 64 in bf16 (494 MB): MEASURED_ROPE.
-constexpr int kRopeBatch = 4;  // heads a thread has in flight
+constexpr int kRopeBatch = 2;  // heads a thread has in flight
 
 template <typename T, int kVec, int kPairing>
 __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeParams p) {
@@ -205,30 +372,9 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeP
                 for (int i = 0; i < kRopeBatch; ++i) {
                     const int head = group + (base + i) * p.groups;
                     if (base + i >= p.per_thread || head >= p.heads) continue;
-                    V u, w;
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) {
-                        // pair e of the chunk: element e of each vector, or
-                        // for neighbours the vectors' elements 2 e, 2 e + 1
-                        if (kPairing != BL_ROPE_ADJACENT) {
-                            const float f = up(a[i].v[e]), g = up(b[i].v[e]);
-                            u.v[e] = down<T>(f * c[e] - g * s[e]);
-                            w.v[e] = down<T>(g * c[e] + f * s[e]);
-                        } else if (kVec == 1) {
-                            const float f = up(a[i].v[0]), g = up(b[i].v[0]);
-                            u.v[0] = down<T>(f * c[0] - g * s[0]);
-                            w.v[0] = down<T>(g * c[0] + f * s[0]);
-                        } else {
-                            const V& in = 2 * e < kVec ? a[i] : b[i];
-                            V& to = 2 * e < kVec ? u : w;
-                            const int k = 2 * e % kVec;
-                            const float f = up(in.v[k]), g = up(in.v[(k + 1) % kVec]);
-                            to.v[k] = down<T>(f * c[e] - g * s[e]);
-                            to.v[(k + 1) % kVec] = down<T>(g * c[e] + f * s[e]);
-                        }
-                    }
-                    *reinterpret_cast<V*>(y + head * p.head_dim + lo) = u;
-                    *reinterpret_cast<V*>(y + head * p.head_dim + hi) = w;
+                    turn_pairs<T, kVec, kPairing == BL_ROPE_ADJACENT>(a[i], b[i], c, s);
+                    *reinterpret_cast<V*>(y + head * p.head_dim + lo) = a[i];
+                    *reinterpret_cast<V*>(y + head * p.head_dim + hi) = b[i];
                 }
             }
         }
@@ -267,7 +413,7 @@ RopeKernel rope_of(int pairing, int vec) {
 int prepare_pack(const bl_pack_args& a, Launch* out) {
     if (a.images == 0 || a.capacity == 0)
         return fail(BL_ERR_INVALID, "pack: no images or no rows");
-    if (a.images > 0x7FFFFFFEu || a.capacity > 0x7FFFFFFFu || a.lead > 0x7FFFFFFFu)
+    if (a.images > 0x7FFFFFFEu || a.capacity > 0x7FFFFFF0u || a.lead > 0x7FFFFFFFu)
         return fail(BL_ERR_UNSUPPORTED, "pack: %u images, %u rows, %u lead rows exceed 32-bit rows",
                     a.images, a.capacity, a.lead);
     if (a.grids == nullptr || a.offsets == nullptr)
@@ -278,16 +424,24 @@ int prepare_pack(const bl_pack_args& a, Launch* out) {
             return fail(BL_ERR_INVALID, "pack: a buffer is not 4-byte aligned");
     Status* st = status_ptr();
     const bl_pack_args b = a;
+    const int vec = ((reinterpret_cast<uintptr_t>(a.image) | reinterpret_cast<uintptr_t>(a.positions)) & 15u) == 0;
     out->op = BL_OP_PACK;
     out->run = [=](cudaStream_t s) {
         const int n = static_cast<int>(b.images), lead = static_cast<int>(b.lead);
-        const long long cap = b.capacity;
+        const int cap = static_cast<int>(b.capacity), norm = b.normalized != 0;
+        const bool maps = b.image != nullptr || b.positions != nullptr;
+        // one thread a group of four rows, at most two blocks an SM (each scans
+        // all sizes again)
+        const unsigned blocks = static_cast<unsigned>(
+            maps ? std::min<uint64_t>((cap + 1023ull) / 1024, 148 * 2) : 1);
+        if (n <= packed::kPackImages)
+            return launch_k(packed::pack_kernel, dim3(blocks), dim3(256), 0, s, b.grids, n, lead,
+                            norm, cap, b.offsets, b.image, b.positions, vec, st);
         cudaError_t e = launch_k(packed::pack_offsets_kernel, dim3(1), dim3(1024), 0, s, b.grids, n,
-                                 lead, cap, b.offsets, st);
-        if (e != cudaSuccess || (b.image == nullptr && b.positions == nullptr)) return e;
-        return launch_k(packed::pack_rows_kernel, dim3(static_cast<unsigned>((cap + 255) / 256)),
-                        dim3(256), 0, s, b.grids, b.offsets, n, lead, static_cast<int>(b.normalized),
-                        cap, b.image, b.positions);
+                                 lead, static_cast<long long>(cap), b.offsets, st);
+        if (e != cudaSuccess || !maps) return e;
+        return launch_k(packed::pack_rows_kernel, dim3(blocks), dim3(256), 0, s, b.grids, b.offsets,
+                        n, lead, norm, cap, b.image, b.positions, vec);
     };
     return BL_OK;
 }
@@ -378,16 +532,21 @@ int prepare_rope(const bl_rope_args& a, Launch* out) {
     };
     while (vec > 1 && !divides(vec)) vec /= 2;
     p.chunks = p.pairs / vec;
-    // Heads a thread turns with one reading of its cosines: four where that
-    // leaves every SM its threads, else one, for the shortest way through.
-    const uint64_t work = 1ull * a.rows * a.heads * p.chunks;
-    const int want = work >= 4ull * 148 * 2048 ? packed::kRopeBatch : 1;
-    p.groups = std::max(1, std::min((p.heads + want - 1) / want, 256 / p.chunks));
-    p.per_thread = (p.heads + p.groups - 1) / p.groups;
-    p.tile_rows = std::max(1, 256 / (p.chunks * p.groups));
-    const uint64_t tiles = (a.rows + p.tile_rows - 1ull) / p.tile_rows;
+    // Heads a thread turns one after the other: one where a block then has one
+    // tile of rows at most (the shortest way through), else up to four, with
+    // as many rows more a tile, so that a tile's barrier and its loads' way
+    // are paid less often. 5477 rows x 16 heads x 80 in f32: MEASURED_HEADS.
+    const unsigned most_blocks = 148 * 8;
+    uint64_t tiles = 0;
+    for (int want = 1; want <= packed::kRopeBatch; want *= 2) {
+        p.groups = std::max(1, std::min((p.heads + want - 1) / want, 256 / p.chunks));
+        p.per_thread = (p.heads + p.groups - 1) / p.groups;
+        p.tile_rows = std::max(1, 256 / (p.chunks * p.groups));
+        tiles = (a.rows + p.tile_rows - 1ull) / p.tile_rows;
+        if (tiles <= most_blocks) break;
+    }
     const size_t smem = 4ull * p.tile_rows * p.pairs * sizeof(float);
-    const unsigned blocks = static_cast<unsigned>(std::min<uint64_t>(tiles, 148 * 8));
+    const unsigned blocks = static_cast<unsigned>(std::min<uint64_t>(tiles, most_blocks));
     const packed::RopeKernel kern = a.dtype == BL_F32   ? packed::rope_of<float>(a.pairing, vec)
                                     : a.dtype == BL_F16 ? packed::rope_of<__half>(a.pairing, vec)
                                                         : packed::rope_of<__nv_bfloat16>(a.pairing, vec);

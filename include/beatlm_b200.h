@@ -522,7 +522,7 @@ int bl_patchify(const bl_patchify_args* args, void* stream);
  */
 typedef struct bl_pack_args {
     uint32_t images;
-    uint32_t capacity;   /* rows of the token buffer, below 2^31 */
+    uint32_t capacity;   /* rows of the token buffer, at most 2^31 - 16 */
     uint32_t lead;
     uint32_t normalized;
     const int32_t* grids;

@@ -44,7 +44,7 @@ def test_pack_matches_the_definition(grids, capacity, lead, normalized):
     assert _status() == 0
 
 
-@pytest.mark.parametrize("images", [31, 32, 33, 1024, 1025, 2500])
+@pytest.mark.parametrize("images", [31, 32, 33, 255, 257, 1024, 1025, 2500, 4096, 4097])
 def test_pack_of_many_images(images):
     rng = np.random.default_rng(images)
     grids = [tuple(int(v) for v in g) for g in rng.integers(0, 6, (images, 3))]
