@@ -826,6 +826,119 @@ class Encoder:
         return sum(2 if isinstance(k.main, PatchEmbed) else 1 for k in prog.kernels)
 
 
+class PackedEncoder:
+    """The encoder's blocks over a packed batch: images and clips of different
+    sizes in one token buffer of ``capacity`` rows, with rotary positions in
+    place of the learned ones (which fit one image size) and attention that
+    keeps to each image. The reference's graph is compiled for one size
+    (depth_anything_v2.rs:435-545) and runs images one after the other.
+
+    Per pass: the batch's row maps from its sizes (``ops.pack``), the patch
+    GEMM, per block LayerNorm, packed Q|K|V GEMM, rotary positions on Q and K
+    in place, attention by image, out-projection, LayerNorm and the MLP's two
+    GEMMs (the block of ``block_specs`` with two kernels more), and the final
+    LayerNorm. Everything is prebuilt once: sizes are device data, so one
+    program (or its graph) runs every batch that fits."""
+
+    def __init__(self, cfg: ViTConfig, weights: dict, capacity: int, images: int,
+                 dtype: str = "bf16", device="cuda", sections=None, theta: float = 100.0,
+                 pairing: str = "axis_half", normalized: bool = False, mask: str | None = None,
+                 cap: float | None = None, slopes=None):
+        """``weights`` as ``Encoder`` takes them (class token and learned
+        positions are not used). ``sections``: rotary pairs of the (time,
+        height, width) axes, default half of the head's pairs for height and
+        half for width; two numbers are (height, width). ``mask``, ``cap`` and
+        ``slopes`` (one a head, a bias by distance on the patch grid): as
+        ``ops.masked_attention``."""
+        import torch
+        if cfg.head_dim != 64:
+            raise ValueError("heads of 64, not %d" % cfg.head_dim)
+        td = torch.bfloat16 if dtype == "bf16" else torch.float16
+        pairs = cfg.head_dim // 2
+        sections = tuple(sections or (pairs // 2, pairs - pairs // 2))
+        if len(sections) not in (2, 3):
+            raise ValueError("rotary sections for (height, width) or (time, height, width)")
+        self.cfg, self.dtype, self.capacity, self.images = cfg, dtype, capacity, images
+        self.blocks = [DeviceBlock(w, cfg.dim, cfg.mlp, dtype, device) for w in weights["blocks"]]
+        f32 = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.float32)).to(device)
+        pw = np.zeros((cfg.dim, cfg.k_pad), np.float32)
+        pw[:, :cfg.taps] = np.asarray(weights["patch_w"], np.float32).reshape(cfg.taps, cfg.dim).T
+        self.patch_w, self.patch_b = torch.from_numpy(pw).to(td).to(device), f32(weights["patch_b"])
+        self.norm = (f32(weights["norm_g"]), f32(weights["norm_b"]))
+        self.slopes = None if slopes is None else f32(slopes)
+        zeros = lambda shape, dt: torch.zeros(shape, dtype=dt, device=device)
+        self.grids = zeros((images, 3), torch.int32)
+        self.offsets = zeros((images + 1,), torch.int32)
+        self.image_of = zeros((capacity,), torch.int32)
+        self.positions = zeros((capacity, 3), torch.float32)
+        self.patches = zeros((capacity, cfg.k_pad), td)
+        self.x = zeros((capacity, cfg.dim), torch.float32)
+        self.xn = zeros((capacity, cfg.dim), td)
+        self.qkv = zeros((capacity, 3 * cfg.dim), torch.int16)
+        # (rows behind the last image are never written: they stay zero)
+        self.o = zeros((capacity, cfg.dim), td)
+        self.h = zeros((capacity, cfg.mlp), td)
+        self.out = zeros((capacity, cfg.dim), torch.float32)
+        self._attention = dict(heads=cfg.heads, qk_dtype=dtype, offsets=self.offsets, out=self.o,
+                               mask=mask, cap=cap, slopes=self.slopes,
+                               positions=None if slopes is None else self.positions)
+        self._rope = dict(sections=sections, theta=theta, pairing=pairing, heads=2 * cfg.heads,
+                          head_dim=cfg.head_dim, dtype=dtype)
+        self._normalized = normalized
+        self._program = None
+
+    def specs(self) -> list:
+        """The pass as kernel specs over this encoder's buffers."""
+        from .runtime import Spec
+        cfg, b = self.cfg, self
+        turn = b.positions[:, 3 - len(b._rope["sections"]):]
+        out = [Spec(ops.pack_args(b.grids, offsets=b.offsets, image=b.image_of,
+                                  positions=b.positions, normalized=b._normalized), "pack"),
+               Spec(_weights_gemm(b.patch_w, a=b.patches, bias=b.patch_b, out=b.x), "embed.patch")]
+        for i, blk in enumerate(self.blocks):
+            ln = lambda w: ops.layernorm_args(b.x, *w, cfg.eps, out=b.xn)
+            block = [
+                (ln(blk.norm1), "norm1"),
+                (_weights_gemm(blk.qkv_w, a=b.xn, bias=blk.qkv_b, out=b.qkv, out_dtype=b.dtype,
+                               out_split=(2 * cfg.dim, "f16")), "qkv"),
+                (ops.rope_args(b.qkv, turn, **b._rope), "rope"),
+                (ops.masked_attention_args(b.qkv, **b._attention), "attention"),
+                (_weights_gemm(blk.proj_w, a=b.o, bias=blk.proj_b, chan_scale=blk.ls1,
+                               residual=b.x, out=b.x), "proj"),
+                (ln(blk.norm2), "norm2"),
+                (_weights_gemm(blk.fc1_w, a=b.xn, bias=blk.fc1_b, act="gelu_erf", out=b.h), "fc1"),
+                (_weights_gemm(blk.fc2_w, a=b.h, bias=blk.fc2_b, chan_scale=blk.ls2,
+                               residual=b.x, out=b.x), "fc2")]
+            out += [Spec(a, "block%d.%s" % (i, name)) for a, name in block]
+        out.append(Spec(ops.layernorm_args(b.x, *b.norm, cfg.eps, out=b.out), "norm"))
+        return out
+
+    def program(self):
+        from .runtime import Kernels
+        if self._program is None:
+            self._program = Kernels(self.specs())
+        return self._program
+
+    def forward(self, patches, grids, stream=None):
+        """``patches``: 16-bit ``[rows][k_pad]`` patch rows (the taps in (ky,
+        kx, ci) order, zero-padded) of the images one after the other;
+        ``grids``: int32 ``[n][3]`` (t, h, w), n at most ``images``. Returns
+        the normalised rows (device f32 ``[capacity][dim]``; image i's are
+        ``offsets[i]`` to ``offsets[i + 1]``, those behind the last hold
+        nothing of use). Nothing waits for the host."""
+        n, rows = grids.shape[0], patches.shape[0]
+        if n > self.images or rows > self.capacity or patches.shape[1] != self.cfg.k_pad:
+            raise ValueError("%d images with %s patch rows in an encoder for %d and [%d][%d]"
+                             % (n, tuple(patches.shape), self.images, self.capacity,
+                                self.cfg.k_pad))
+        with _on_stream(stream):
+            self.grids[:n].copy_(grids)
+            self.grids[n:].zero_()
+            self.patches[:rows].copy_(patches)
+            self.program().encode_all(None)
+        return self.out
+
+
 class HostPipeline:
     """Frames from pinned host memory to pinned host memory over two input/
     output slots (the reference keeps jobs in flight through its Net slots,
