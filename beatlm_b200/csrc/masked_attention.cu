@@ -423,7 +423,24 @@ static_assert(kColO + HD <= kTmemCols, "TMEM columns");
 // O is rescaled: P stays below 2^8, well inside f16.
 constexpr float kRescaleThreshold = 8.0f;
 
+// The bias of |i - j| comes out of the tensor cores where it is linear over a
+// tile, that is where every key that any row of the CTA sees lies on one side
+// of the row: it is then lean (k - rel) for key k of the tile, and one more K
+// step of the product S adds (slope / scale) k to every score, with the
+// operands below; -lean rel is the row's and goes into its exponents' offset.
+// So a linear tile costs the softmax nothing. Both halves of the K step hold
+// the same (half of the slope each), so the swizzle does not matter; the slope
+// is the sum of three bf16 values (24 bits), the key's number is exact.
+struct LeanOperands {
+    uint8_t slope[BM * 32];      // A: every row the slope's three parts, twice
+    uint8_t key[2][BN * 32];     // B: row k holds k (or -k) three times, twice
+};
+
 struct TileTail {
+    alignas(1024) union {
+        LeanOperands lean;
+        float kpos[8][3][BN];  // each softmax warp's copy of a key tile's positions
+    };
     uint64_t q_full;
     uint64_t kv_full[STAGES];
     uint64_t kv_empty[STAGES];
@@ -444,10 +461,17 @@ struct TileTail {
     int t0, n;      // its key tiles
     float ref[2][BM];      // R after the stream's last tile
     float odd_sum[BM];
-    alignas(16) float kpos[8][3][BN];  // each softmax warp's copy of a key tile's positions
 };
 constexpr size_t kTileSmem = 1024 + kQBytes + 2 * STAGES * kKvBytes + sizeof(TileTail);
 static_assert(2 * (kTileSmem + 1024) <= 233472, "two CTAs an SM");
+
+// On which side of all the CTA's rows the keys of the tile at k0 lie that any of
+// them sees: 1 before, -1 behind, 0 on both. Under a causal mask, and behind a
+// prefix, no row sees a key behind itself.
+__device__ __forceinline__ int side_of(const Params& p, int prefix, int q0, int k0) {
+    if (k0 + BN - 1 <= q0 || (p.mask != BL_MASK_NONE && k0 >= prefix)) return 1;
+    return k0 >= q0 + BM - 1 ? -1 : 0;
+}
 
 // The sequence (its rows, without the prefix) and tile of tile `index` of the
 // packed batch, the longest sequences' tiles first while there are at most 32
@@ -656,6 +680,19 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
         __syncwarp();
     }
+    if (kBias == BIAS_INDEX && !kCap && warp >= kSoftmaxWarp0) {
+        // 256 threads, 256 16-byte parts of A and as many of the two B
+        const int t = threadIdx.x - 32 * kSoftmaxWarp0;
+        const float half = 0.5f * p.slopes[head] / p.scale;
+        const float a = __bfloat162float(__float2bfloat16_rn(half));
+        const float b = __bfloat162float(__float2bfloat16_rn(half - a));
+        reinterpret_cast<uint4*>(tail->lean.slope)[t] =
+            make_uint4(pack_bf16x2(a, b), pack_bf16x2(half - a - b, 0.0f), 0, 0);
+        const float k = static_cast<float>((t & 127) >> 1), e = t < 128 ? k : -k;
+        reinterpret_cast<uint4*>(tail->lean.key)[t] =
+            make_uint4(pack_bf16x2(e, e), pack_bf16x2(e, 0.0f), 0, 0);
+        fence_proxy_async_smem();
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -715,7 +752,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         // operand, one swizzle atom wide, groups of 8 keys 1024 bytes apart
         const uint64_t dv = sdesc_sw128(smem_u32(sV), kKvBytes, 1024);
         constexpr uint64_t kStep = kKvBytes >> 4;
-        const int end = tail->span.len;
+        const int end = tail->span.len, prefix = tail->span.prefix, q0 = tail->q0;
+        const uint32_t idesc_lean = idesc_f16(BM, BN, 1, 1, 0, 0);
+        const uint64_t d_slope = sdesc_sw32(smem_u32(tail->lean.slope), 256);
+        const uint64_t d_key = sdesc_sw32(smem_u32(tail->lean.key), 256);
         // ring places, stepped as the loop goes: S runs SBUFS tiles ahead of PV
         int sb = 0, st = 0, st_phase = 0;  // of the next S: TMEM buffer, stage
         int pb = 0, p_phase = 0, pt = 0;   // of the next PV
@@ -734,13 +774,17 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             }
             return true;
         };
-        auto issue_s = [&]() {
+        auto issue_s = [&](int i) {
+            const int side = kBias == BIAS_INDEX && !kCap ? side_of(p, prefix, q0, (t0 + i) * BN) : 0;
             const uint64_t b = dk + st * kStep;
             const uint32_t dst = tmem + BN * sb;
             if (elected) {
                 mma_ss(dst, dq, b, idesc_s, 0u);
 #pragma unroll
                 for (int k = 1; k < HD / 16; ++k) mma_ss(dst, dq + 2 * k, b + 2 * k, idesc_s, 1u);
+                if (side != 0)
+                    mma_ss(dst, d_slope, d_key + (side < 0 ? sizeof(tail->lean.key[0]) >> 4 : 0),
+                           idesc_lean, 1u);
                 mma_commit(smem_u32(&tail->s_full[sb]));
             }
             __syncwarp();
@@ -766,7 +810,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         for (int i = 0; i < SBUFS && i < n && ok; ++i) {
             ok = wait_tile(i);
             tc_fence_after();
-            if (ok) issue_s();
+            if (ok) issue_s(i);
         }
         for (int i = 0; i < n && ok; ++i) {
             // what S(i + 3) needs first: between P(i) and it stand only MMAs
@@ -776,7 +820,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             if (!ok) break;
             tc_fence_after();
             issue_pv(i);
-            if (more) issue_s();
+            if (more) issue_s(i + SBUFS);
         }
         if (!ok) {
             // unwinding: what was issued completes before TMEM is released
@@ -849,18 +893,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             // some row of the warp sees less than the whole tile
             const bool cut = __any_sync(kFull, valid < BN);
             const float rel = static_cast<float>(at - k0);
-            // |i - j| is linear over the tile where all its keys lie on one
-            // side of all the warp's rows: the bias of key k is then
-            // lean (k - rel), and takes part in the scaling's FMA
-            const int row0 = tail->q0 + sub * 32;
-            const bool before = k0 + BN - 1 <= row0, after = k0 >= row0 + 31;
-            const bool linear = kBias == BIAS_INDEX && !kCap && (before || after);
-            const float lean = before ? slope2 : -slope2;
-            // the biases of keys k and k + 1, formed anew every eighth key
-            auto lean2 = [&](int k, float less) {
-                const float b = fmaf(lean, static_cast<float>(k) - rel, -less);
-                return f2pack(b, b + lean);
-            };
+            // a linear bias (side_of): what is left of it is the row's
+            const int side = kBias == BIAS_INDEX && !kCap ? side_of(p, q.prefix, tail->q0, k0) : 0;
+            const bool linear = side != 0;
+            const float lean = linear ? -static_cast<float>(side) * slope2 * rel : 0.0f;
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             float far = 0.0f;  // the largest |score|, for the capping's choice
             bool small = false;
@@ -888,15 +924,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                     far = fmax3(fmaxf(far, f[0]), fmaxf(f[1], f[2]), f[3]);
                     small = !__any_sync(kFull, far * cap.unit > kSmallTanh);
                 }
-                if (linear) {
-                    unsigned long long b = 0;
-                    const unsigned long long step = both(2.0f * lean), in2 = both(in);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        b = e % 4 == 0 ? lean2(32 * h + 2 * e, 0.0f) : fadd2(b, step);
-                        set(e, ffma2(pair(e), in2, b));
-                    }
-                } else if (kBias != BIAS_NONE) {
+                if (kBias != BIAS_NONE && !linear) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int k = 32 * h + 2 * e;
@@ -938,6 +966,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             if (kBias != BIAS_NONE && !linear) tmem_wait_st();
             float m_row = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
             if (kPlain) m_row *= in;
+            if (linear) m_row = fmaf(m_row, in, lean);
             // (capping keeps the order: the largest capped score is the capped
             // largest)
             if (kCapOnly && m_row != -INFINITY)
@@ -1017,13 +1046,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) finish(e, ffma2(pair(e), both(in), nm2));
                 } else if (kBias == BIAS_INDEX && linear) {
-                    const unsigned long long in2 = both(in), step = both(2.0f * lean);
-                    unsigned long long b = 0;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        b = e % 4 == 0 ? lean2(32 * h + 2 * e, -nm) : fadd2(b, step);
-                        finish(e, ffma2(pair(e), in2, b));
-                    }
+                    for (int e = 0; e < 16; ++e) finish(e, ffma2(pair(e), both(in), both(nm + lean)));
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) finish(e, fadd2(pair(e), nm2));
