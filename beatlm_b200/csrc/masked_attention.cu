@@ -412,6 +412,7 @@ constexpr int BM = 128;
 constexpr int BN = 64;
 constexpr int STAGES = 5;  // K/V ring
 constexpr int SBUFS = 3;
+constexpr unsigned kSms = 148;
 constexpr int kTileThreads = 320;  // two CTAs of 96 registers a thread
 constexpr int kSoftmaxWarp0 = 2;
 constexpr uint32_t kQBytes = BM * HD * 2;
@@ -439,7 +440,7 @@ struct LeanOperands {
 struct TileTail {
     alignas(1024) union {
         LeanOperands lean;
-        float kpos[8][3][BN];  // each softmax warp's copy of a key tile's positions
+        float kpos[8][3][BN];  // each softmax warp's copy of a key tile's positions, negated
     };
     uint64_t q_full;
     uint64_t kv_full[STAGES];
@@ -570,33 +571,58 @@ __device__ __forceinline__ void store8(void* out, long long at, int dt, const fl
 }
 
 // cap tanh(s / cap) of two raw scores in log2 units. Where every |u| = |s / cap|
-// of the warp's tile is at most kSmallTanh, by the odd series through u^9 on
-// the FMA units (the first term left out is below 10^-6 of the value there),
-// which spares the unit that the exponentials need two of its three functions
-// a score; otherwise by those.
-constexpr float kSmallTanh = 0.4f;
+// of the warp's tile is at most kSmallTanh, by the odd series through u^7 on
+// the FMA units (the first term left out is below 4 10^-7 of the value there),
+// as s times a cubic in s^2: that spares the unit that the exponentials need
+// two of its three functions a score. Otherwise by those.
+constexpr float kSmallTanh = 0.25f;
 struct Capping {
     float unit;   // raw score -> u
-    float scale;  // raw score -> log2 units, uncapped
+    float c[4];   // the series' coefficients for raw scores, in log2 units
     float twice;  // raw score -> 2 u in log2 units
     float cap2;   // cap in log2 units
+    __device__ explicit Capping(const Params& p)
+        : unit(p.scale / p.cap), twice(2.0f * unit * kLog2e), cap2(p.cap * kLog2e) {
+        const float v = unit * unit;
+        c[0] = p.scale * kLog2e;
+        c[1] = c[0] * v * (-1.0f / 3.0f);
+        c[2] = c[0] * v * v * (2.0f / 15.0f);
+        c[3] = c[0] * v * v * v * (-17.0f / 315.0f);
+    }
 };
 __device__ __forceinline__ unsigned long long both(float v) { return f2pack(v, v); }
-__device__ __forceinline__ unsigned long long capped2(unsigned long long s, const Capping& k,
-                                                      bool small) {
-    if (small) {
-        const unsigned long long u = fmul2(s, both(k.unit)), v = fmul2(u, u);
-        unsigned long long c = ffma2(v, both(62.0f / 2835.0f), both(-17.0f / 315.0f));
-        c = ffma2(v, c, both(2.0f / 15.0f));
-        c = ffma2(v, c, both(-1.0f / 3.0f));
-        const unsigned long long w = fmul2(s, both(k.scale));
-        return ffma2(fmul2(w, v), c, w);
+template <bool kSmall>
+__device__ __forceinline__ unsigned long long capped2(unsigned long long s, const Capping& k) {
+    if (kSmall) {
+        const unsigned long long z = fmul2(s, s);
+        unsigned long long c = ffma2(z, both(k.c[3]), both(k.c[2]));
+        c = ffma2(z, c, both(k.c[1]));
+        c = ffma2(z, c, both(k.c[0]));
+        return fmul2(s, c);
     }
     float a, b;
     f2unpack(s, a, b);
     a = fmaf(rcp_approx(1.0f + ex2(a * k.twice)), -2.0f * k.cap2, k.cap2);
     b = fmaf(rcp_approx(1.0f + ex2(b * k.twice)), -2.0f * k.cap2, k.cap2);
     return f2pack(a, b);
+}
+// 32 raw scores capped in place. (A branch around each loop: inside it the two
+// forms would both be computed.)
+__device__ __forceinline__ void cap32(uint32_t (&s)[32], const Capping& k, bool small) {
+    auto put = [&](int e, unsigned long long v) {
+        float x, y;
+        f2unpack(v, x, y);
+        s[2 * e] = __float_as_uint(x), s[2 * e + 1] = __float_as_uint(y);
+    };
+    if (small) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            put(e, capped2<true>(f2pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), k));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            put(e, capped2<false>(f2pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), k));
+    }
 }
 
 enum { BIAS_NONE = 0, BIAS_INDEX = 1, BIAS_PLANE = 2, BIAS_SPACE = 3 };
@@ -617,8 +643,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     // CTAs in the order of their start: the splits of a unit side by side (a
     // cluster), then the heads of a tile, so that the tiles with most keys (the
     // first units) start first in every head and the last CTAs are short
-    const unsigned work = blockIdx.x / static_cast<unsigned>(p.splits);
+    unsigned work = blockIdx.x / static_cast<unsigned>(p.splits);
     const unsigned split = blockIdx.x - work * p.splits;
+    // (one CTA an SM goes out before any SM gets its second: where all fit at
+    // once, the second ones come lightest first, beside the heaviest)
+    if (p.splits == 1 && gridDim.x <= 2 * kSms && work >= kSms) work = gridDim.x - 1 - (work - kSms);
     const int unit = static_cast<int>(work / static_cast<unsigned>(p.heads));
     const int head = static_cast<int>(work - static_cast<unsigned>(unit) * p.heads);
     const int kvh = head / p.group;
@@ -856,22 +885,20 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         constexpr bool kCapOnly = kCap && kBias == BIAS_NONE;
         // raw scores to log2 units; kPlain does it in the exponent's FMA
         const float in = p.scale * kLog2e;
-        const Capping cap{kCap ? p.scale / p.cap : 0.0f, in, kCap ? 2.0f * p.scale / p.cap * kLog2e : 0.0f,
-                          p.cap * kLog2e};
+        const Capping cap(p);  // (read under kCap alone)
         const float slope2 = kBias != BIAS_NONE ? p.slopes[head] * kLog2e : 0.0f;
-        float qp[3] = {0.0f, 0.0f, 0.0f};
-        if (kBias >= BIAS_PLANE) {
+        constexpr int kAxes = kBias == BIAS_SPACE ? 3 : 2;
+        unsigned long long qp2[kAxes];  // this row's place, twice
 #pragma unroll
-            for (int a = 0; a < 3; ++a)
-                if (live && a < p.pos_axes) qp[a] = p.pos[(q.begin + at) * p.pos_row + a];
-        }
+        for (int a = 0; a < kAxes; ++a)
+            qp2[a] = both(kBias >= BIAS_PLANE && live && a < p.pos_axes
+                              ? p.pos[(q.begin + at) * p.pos_row + a] : 0.0f);
         const float(*kpos)[BN] = tail->kpos[warp - kSoftmaxWarp0];
         float m_used = -INFINITY, l = 0.0f;  // R as this thread last knew it; l is relative to it
         bool ok = true;
         // tile i: S buffer `buf` = i % SBUFS, whose use it is the phase of
         int buf = odd, phase = 0;
         // the positions of this lane's two keys of the next tile
-        constexpr int kAxes = kBias == BIAS_SPACE ? 3 : 2;
         float ahead[kAxes][2];
         auto fetch = [&](int i) {
 #pragma unroll
@@ -892,7 +919,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 for (int a = 0; a < kAxes; ++a)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        tail->kpos[warp - kSoftmaxWarp0][a][lane + 32 * e] = ahead[a][e];
+                        tail->kpos[warp - kSoftmaxWarp0][a][lane + 32 * e] = -ahead[a][e];
                 __syncwarp();
                 fetch(i + 2);
             }
@@ -936,29 +963,36 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                     small = !__any_sync(kFull, far * cap.unit > kSmallTanh);
                 }
                 if (kBias != BIAS_NONE && !linear) {
+                    const unsigned long long down = both(-slope2);
+                    if (kCap) cap32(s, cap, small);
+                    auto score = [&](int e) { return kCap ? pair(e) : fmul2(pair(e), both(in)); };
+                    if (kBias == BIAS_INDEX) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int k = 32 * h + 2 * e;
-                        unsigned long long t = kCap ? capped2(pair(e), cap, small)
-                                                    : fmul2(pair(e), both(in));
-                        unsigned long long d;
-                        if (kBias == BIAS_INDEX) {
-                            d = f2pack(fabsf(rel - static_cast<float>(k)),
-                                       fabsf(rel - static_cast<float>(k + 1)));
-                        } else {
-                            // the distance from each key's copy of its place
-                            unsigned long long d2 = 0;
-#pragma unroll
-                            for (int a = 0; a < (kBias == BIAS_SPACE ? 3 : 2); ++a) {
-                                const float2 w = *reinterpret_cast<const float2*>(&kpos[a][k]);
-                                const unsigned long long x = fadd2(both(qp[a]), f2pack(-w.x, -w.y));
-                                d2 = a == 0 ? fmul2(x, x) : ffma2(x, x, d2);
-                            }
-                            float x, y;
-                            f2unpack(d2, x, y);
-                            d = f2pack(sqrt_approx(x), sqrt_approx(y));
+                        for (int e = 0; e < 16; ++e) {
+                            const float k = static_cast<float>(32 * h + 2 * e);
+                            set(e, ffma2(down, f2pack(fabsf(rel - k), fabsf(rel - k - 1.0f)), score(e)));
                         }
-                        set(e, ffma2(both(-slope2), d, t));
+                    } else {
+                        // distances from the keys' places, four keys a load
+                        auto root = [](unsigned long long v) {
+                            float x, y;
+                            f2unpack(v, x, y);
+                            return f2pack(sqrt_approx(x), sqrt_approx(y));
+                        };
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            unsigned long long d0 = 0, d1 = 0;
+#pragma unroll
+                            for (int a = 0; a < kAxes; ++a) {
+                                const float4 w = *reinterpret_cast<const float4*>(&kpos[a][32 * h + 2 * e]);
+                                const unsigned long long x0 = fadd2(qp2[a], f2pack(w.x, w.y));
+                                const unsigned long long x1 = fadd2(qp2[a], f2pack(w.z, w.w));
+                                d0 = a == 0 ? fmul2(x0, x0) : ffma2(x0, x0, d0);
+                                d1 = a == 0 ? fmul2(x1, x1) : ffma2(x1, x1, d1);
+                            }
+                            set(e, ffma2(down, root(d0), score(e)));
+                            set(e + 1, ffma2(down, root(d1), score(e + 1)));
+                        }
                     }
                 }
                 if (cut) {
@@ -1028,15 +1062,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 uint32_t s[32];
                 tmem_ld32(s_col + 32 * h, s);
                 tmem_wait_ld();
-                if (kCapOnly) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float x, y;
-                        f2unpack(capped2(f2pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])),
-                                         cap, small), x, y);
-                        s[2 * e] = __float_as_uint(x), s[2 * e + 1] = __float_as_uint(y);
-                    }
-                }
+                if (kCapOnly) cap32(s, cap, small);
                 // (scores stored back in the first pass are masked already)
                 if ((kPlain || kCapOnly || linear) && cut) {
 #pragma unroll
