@@ -89,22 +89,24 @@ __device__ __forceinline__ float sqrt_approx(float x) {
 //
 // The newest rows of a stream: up to 16 query rows of one K/V head (rows and
 // heads of its group alike), for which the keys' bytes are what counts. Each
-// of a CTA's four warps walks its own 16-key tiles of one split of the keys,
-// with three tiles on their way to a shared-memory ring of its own (12 KB a
-// warp in flight, 12 warps an SM; no barrier between warps). 16 rows are the
+// of a CTA's four warps walks its own 32-key tiles of one split of the keys,
+// with two tiles on their way to a shared-memory ring of its own (16 KB a warp
+// in flight; no barrier between warps). 16 rows are the
 // smallest tile of the warp-level tensor instruction (m16n8k16), which takes
-// S = Q K^T and O += P V of a tile in 16 instructions, so the arithmetic stays
-// below the bytes: on the FMA units one row alone cost 400 instructions a
-// tile. Scores, maxima, sums and O are f32, P is rounded to f16 (it is at most
-// 1: the running maximum is exact here). Warps, then the cluster's CTAs, are
-// merged once at the end, in rank order.
+// S = Q K^T and O += P V of 16 keys in 16 instructions, so the arithmetic stays
+// below the bytes: on the FMA units one row alone cost 400 instructions
+// for 16 keys. Scores, maxima, sums and O are f32, P is rounded to f16 (it is at most
+// 1: the running maximum is exact here). Warps
+// are merged once at the end; the CTAs of a cluster send their rows' parts into
+// the first one's shared memory and leave, and that adds them in rank order.
 // MEASURED_TOKEN
 constexpr int kRowWarps = 4;
-constexpr int kRowTile = 16;    // keys of a tile
-constexpr int kRowStages = 4;
+constexpr int kRowTile = 32;    // keys of a tile
+constexpr int kRowStages = 2;
 constexpr int kMaxRows = 16;    // query rows of a CTA
 constexpr int kRowTileBytes = 2 * kRowTile * HD * 2;  // K, then V
-constexpr size_t kRowSmem = kRowWarps * kRowStages * kRowTileBytes;
+constexpr size_t kRowRing = kRowWarps * kRowStages * kRowTileBytes;
+constexpr int kPartFloats = HD + 2;  // a row's O, maximum and sum from another split
 static_assert(kRowStages * kRowTileBytes >= kMaxRows * HD * 4, "a warp's O over its ring");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
@@ -141,17 +143,61 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
     pdl_wait();
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float2 part_ml[kRowWarps][kMaxRows];
-    __shared__ float cta_o[kMaxRows][HD];
-    __shared__ float2 cta_ml[kMaxRows];
+    __shared__ uint64_t parts_full;
+    float* parts = reinterpret_cast<float*>(ring + kRowRing);  // [split][row][kPartFloats]
     constexpr unsigned kFull = 0xFFFFFFFFu;
     const int warp = warp_id(), lane = lane_id();
-    const int split = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.splits));
-    const int unit = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.splits));
+    // The heads of the same keys start side by side: their 128-byte parts of
+    // a packed row are neighbours, so memory pages are read while they are open.
+    const unsigned work = blockIdx.x / static_cast<unsigned>(p.splits);
+    const int split = static_cast<int>(blockIdx.x - work * p.splits);
+    const int unit = static_cast<int>(work / static_cast<unsigned>(p.kv_heads));
+    const int kvh = static_cast<int>(work - static_cast<unsigned>(unit) * p.kv_heads);
     const int c0 = unit % p.chunks * kMaxRows;
     const Span q = span_of(p, unit / p.chunks);
-    const int kvh = blockIdx.y;
     const int rows = min((q.len - q.first) * p.group - c0, kMaxRows);
     if (rows <= 0) return;  // the whole cluster leaves
+    if (p.splits > 1) {
+        if (threadIdx.x == 0) {
+            mbar_init(smem_u32(&parts_full), p.splits - 1);
+            fence_barrier_init();
+        }
+        __syncwarp();
+        cluster_arrive();  // waited for before the parts are sent
+    }
+
+    const int most = visible(p, q, q.first + (c0 + rows - 1) / p.group);  // of the last row
+    const int least = visible(p, q, q.first + c0 / p.group);               // of the first
+    const int tiles = (most + kRowTile - 1) / kRowTile;
+    const int first = static_cast<int>(static_cast<unsigned>(tiles) * split / p.splits);
+    const int last = static_cast<int>(static_cast<unsigned>(tiles) * (split + 1) / p.splits);
+
+    // A lane copies one 16-byte part of every fourth key of a tile. A key row is
+    // 128 bytes: its eight parts are rotated by the row, so that the matrix
+    // loads meet no bank twice; (4 i + r) & 7 is r or r ^ 4.
+    const int lr = lane >> 3, lp = lane & 7;
+    const uint16_t* src = p.qkv + (q.begin + (first + warp) * kRowTile + lr) * p.row +
+                          (p.heads + kvh) * HD + lp * 8;
+    const long long to_v = static_cast<long long>(p.kv_heads) * HD, four = 4 * p.row;
+    const uint32_t mine = smem_u32(ring) + warp * kRowStages * kRowTileBytes;
+    const uint32_t at0 = lr * 128 + ((lp ^ lr) << 4), at1 = lr * 128 + ((lp ^ lr ^ 4) << 4);
+    auto fetch = [&](int tile, int stage) {
+        if (tile < last) {
+            const uint32_t dst = mine + stage * kRowTileBytes;
+            const int left = most - tile * kRowTile - lr;  // this lane's keys before the end
+#pragma unroll
+            for (int i = 0; i < kRowTile / 4; ++i) {
+                const uint32_t at = dst + i * 512 + (i % 2 == 0 ? at0 : at1);
+                const bool real = 4 * i < left;
+                const uint16_t* from = real ? src + i * four : p.qkv;
+                cp_async16(at, from, real);
+                cp_async16(at + kRowTile * 128, real ? from + to_v : p.qkv, real);
+            }
+            src += kRowWarps * kRowTile / 4 * four;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int i = 0; i < kRowStages - 1; ++i) fetch(first + warp + i * kRowWarps, i);
 
     // This thread's two query rows (of the 16: g and g + 8), as the products'
     // accumulators hold them; a row past the last repeats it and is not stored.
@@ -177,30 +223,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
             qp[r][a] = p.pos != nullptr && a < p.pos_axes
                            ? p.pos[(q.begin + row[r]) * p.pos_row + a] : 0.0f;
     }
-    const int most = visible(p, q, q.first + (c0 + rows - 1) / p.group);  // of the last row
-    const int tiles = (most + kRowTile - 1) / kRowTile;
-    const int first = static_cast<int>(static_cast<unsigned>(tiles) * split / p.splits);
-    const int last = static_cast<int>(static_cast<unsigned>(tiles) * (split + 1) / p.splits);
-
-    const uint16_t* kbase = p.qkv + q.begin * p.row + (p.heads + kvh) * HD + (lane & 7) * 8;
-    const long long to_v = static_cast<long long>(p.kv_heads) * HD;
-    const uint32_t mine = smem_u32(ring) + warp * kRowStages * kRowTileBytes;
-    auto fetch = [&](int tile, int stage) {
-        if (tile < last) {
-            const uint32_t dst = mine + stage * kRowTileBytes;
-#pragma unroll
-            for (int i = 0; i < kRowTile / 4; ++i) {
-                const int k = 4 * i + (lane >> 3), key = tile * kRowTile + k;
-                // a key row is 128 bytes: its eight 16-byte parts rotated by
-                // the row, so that the matrix loads meet no bank twice
-                const uint32_t at = dst + k * 128 + (((lane & 7) ^ (k & 7)) << 4);
-                const uint16_t* src = kbase + min(key, most - 1) * p.row;
-                cp_async16(at, src, key < most);
-                cp_async16(at + kRowTile * 128, src + to_v, key < most);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     float o[HD / 8][4];
 #pragma unroll
     for (int d = 0; d < HD / 8; ++d)
@@ -211,7 +233,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
     const float in = capped_scores ? 2.0f * p.scale / p.cap * kLog2e : p.scale * kLog2e;
     const float cap2 = p.cap * kLog2e;
 
-    for (int i = 0; i < kRowStages - 1; ++i) fetch(first + warp + i * kRowWarps, i);
     int stage = 0;
     for (int tile = first + warp; tile < last; tile += kRowWarps) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 2) : "memory");
@@ -221,52 +242,69 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
         const uint32_t sk = mine + stage * kRowTileBytes, sv = sk + kRowTile * 128;
         stage = (stage + 1) % kRowStages;
         const int base = tile * kRowTile;
-        float s[2][4];
+        // s[t][2 r + e]: query row g + 8 r, key base + 8 t + 2 quad + e
+        constexpr int T = kRowTile / 8;
+        float s[T][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-            // keys 0..7 and 8..15 by the two halves of 16 columns
-            uint32_t b[4];
-            const int key = (lane >> 4) * 8 + (lane & 7), part = 2 * k + ((lane >> 3) & 1);
-            ldmatrix4(sk + key * 128 + ((part ^ (key & 7)) << 4), b);
-            mma16<kBf16>(s[0], qa[k], b[0], b[1]);
-            mma16<kBf16>(s[1], qa[k], b[2], b[3]);
-        }
-        // s[t][2 r + e]: query row g + 8 r, key base + 8 t + 2 quad + e
-        float top[2] = {-INFINITY, -INFINITY};
+        for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int key = base + 8 * t + 2 * quad + e;
-                float kp[3] = {0.0f, 0.0f, 0.0f};
-                if (p.pos != nullptr) {
-#pragma unroll
-                    for (int a = 0; a < 3; ++a)
-                        if (key < most && a < p.pos_axes) kp[a] = p.pos[(q.begin + key) * p.pos_row + a];
-                }
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float x = s[t][2 * r + e] * in;
-                    if (capped_scores) x = fmaf(rcp_approx(1.0f + ex2(x)), -2.0f * cap2, cap2);
-                    if (p.slopes != nullptr) {
-                        float far = fabsf(static_cast<float>(row[r] - key));
-                        if (p.pos != nullptr) {
-                            const float dx = qp[r][0] - kp[0], dy = qp[r][1] - kp[1],
-                                        dz = qp[r][2] - kp[2];
-                            far = sqrt_approx(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
-                        }
-                        x = fmaf(-slope[r], far, x);
-                    }
-                    x = key < seen[r] ? x : -INFINITY;
-                    s[t][2 * r + e] = x;
-                    top[r] = fmaxf(top[r], x);
-                }
+            for (int t = 0; t < T; t += 2) {
+                // eight keys, then eight, by the two halves of 16 columns
+                uint32_t b[4];
+                const int key = 8 * t + (lane >> 4) * 8 + (lane & 7);
+                const int part = 2 * k + ((lane >> 3) & 1);
+                ldmatrix4(sk + key * 128 + ((part ^ (key & 7)) << 4), b);
+                mma16<kBf16>(s[t], qa[k], b[0], b[1]);
+                mma16<kBf16>(s[t + 1], qa[k], b[2], b[3]);
             }
-        uint32_t pa[4];
+        auto each = [&](auto&& f) {  // f(score, its row of the two, its key - base - 2 quad)
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][e] = f(s[t][e], e >> 1, 8 * t + (e & 1));
+        };
+        if (capped_scores)
+            each([&](float x, int, int) {
+                return fmaf(rcp_approx(1.0f + ex2(x * in)), -2.0f * cap2, cap2);
+            });
+        else
+            each([&](float x, int, int) { return x * in; });
+        const int own = base + 2 * quad;  // this lane's first key
+        if (p.slopes != nullptr) {
+            if (p.pos == nullptr) {
+                const float rel[2] = {static_cast<float>(row[0] - own), static_cast<float>(row[1] - own)};
+                each([&](float x, int r, int k) {
+                    return fmaf(-slope[r], fabsf(rel[r] - static_cast<float>(k)), x);
+                });
+            } else {
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = min(own + 8 * t + e, most - 1);
+                        float d2[2] = {0.0f, 0.0f};
+                        for (int a = 0; a < p.pos_axes; ++a) {
+                            const float kp = p.pos[(q.begin + key) * p.pos_row + a];
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float d = (a == 0 ? qp[r][0] : a == 1 ? qp[r][1] : qp[r][2]) - kp;
+                                d2[r] = fmaf(d, d, d2[r]);
+                            }
+                        }
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            s[t][2 * r + e] = fmaf(-slope[r], sqrt_approx(d2[r]), s[t][2 * r + e]);
+                    }
+            }
+        }
+        if (base + kRowTile > least)  // some row sees less than the whole tile
+            each([&](float x, int r, int k) { return own + k < seen[r] ? x : -INFINITY; });
+        float top[2] = {-INFINITY, -INFINITY};
+        each([&](float x, int r, int) { top[r] = fmaxf(top[r], x); return x; });
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             top[r] = fmaxf(top[r], __shfl_xor_sync(kFull, top[r], 1));
@@ -283,24 +321,27 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
                 for (int d = 0; d < HD / 8; ++d) o[d][2 * r] *= shrink, o[d][2 * r + 1] *= shrink;
             }
         }
+        // (no key seen yet: against 0)
+        const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+        each([&](float x, int r, int) {
+            const float v = ex2(x - ref[r]);
+            l[r] += v;
+            return v;
+        });
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float ref = m[r] == -INFINITY ? 0.0f : m[r];  // no key seen yet
+        for (int t = 0; t < T; t += 2) {
+            const uint32_t pa[4] = {pack_f16x2(s[t][0], s[t][1]), pack_f16x2(s[t][2], s[t][3]),
+                                    pack_f16x2(s[t + 1][0], s[t + 1][1]),
+                                    pack_f16x2(s[t + 1][2], s[t + 1][3])};
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const float a = ex2(s[t][2 * r] - ref), b = ex2(s[t][2 * r + 1] - ref);
-                l[r] += a + b;
-                pa[2 * t + r] = pack_f16x2(a, b);
+            for (int d = 0; d < HD / 16; ++d) {
+                // keys 8 t.. and 8 t + 8.. of columns 16 d.., then of the next 8
+                uint32_t b[4];
+                const int key = 8 * t + (lane & 15), part = 2 * d + (lane >> 4);
+                ldmatrix4_trans(sv + key * 128 + ((part ^ (key & 7)) << 4), b);
+                mma16<false>(o[2 * d], pa, b[0], b[1]);
+                mma16<false>(o[2 * d + 1], pa, b[2], b[3]);
             }
-        }
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) {
-            // keys 0..7 and 8..15 of columns 16 d..16 d + 7, then of the next 8
-            uint32_t b[4];
-            const int key = lane & 15, part = 2 * d + (lane >> 4);
-            ldmatrix4_trans(sv + key * 128 + ((part ^ (key & 7)) << 4), b);
-            mma16<false>(o[2 * d], pa, b[0], b[1]);
-            mma16<false>(o[2 * d + 1], pa, b[2], b[3]);
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -326,7 +367,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
         else if (p.out_dtype == BL_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
         else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
     };
-    // warps -> CTA
+    if (p.splits > 1) cluster_wait();  // the first CTA is there
+    // warps -> CTA, and to the cluster's first one
     for (int t = threadIdx.x; t < rows * HD; t += 32 * kRowWarps) {
         const int r = t / HD, e = t % HD;
         float best = -INFINITY, v = 0.0f, sum = 0.0f;
@@ -341,43 +383,36 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
         }
         if (p.splits == 1) {
             put(r, e, v / sum);
-        } else {
-            cta_o[r][e] = v;
-            if (e == 0) cta_ml[r] = make_float2(best, sum);
+            continue;
         }
+        const uint32_t to = dsmem_addr(smem_u32(parts + (split * rows + r) * kPartFloats), 0);
+        dsmem_st1(to + 4 * e, v);
+        if (e == 0) dsmem_st2(to + 4 * HD, best, sum);
     }
     if (p.splits == 1) return;
-    __syncthreads();
     fence_cluster();
-    cluster_sync();
-    // CTAs -> rows: the cluster's CTAs share out the values
-    for (int t = split * 32 * kRowWarps + threadIdx.x; t < rows * HD; t += p.splits * 32 * kRowWarps) {
+    __syncthreads();
+    if (split != 0) {
+        if (threadIdx.x == 0)
+            mbar_arrive_remote(dsmem_addr(smem_u32(&parts_full), 0));
+        return;
+    }
+    if (!mbar_wait_cluster(smem_u32(&parts_full), 0, nullptr, p.status, ST_TIMEOUT_SOFTMAX, 0x50000))
+        return;
+    for (int t = threadIdx.x; t < rows * HD; t += 32 * kRowWarps) {
         const int r = t / HD, e = t % HD;
-        float2 ml[8];
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k)  // every load on its way before the first use
-            if (k < p.splits) {
-                ml[k] = dsmem_ld2(dsmem_addr(smem_u32(&cta_ml[r]), k));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[k])
-                             : "r"(dsmem_addr(smem_u32(&cta_o[r][e]), k)));
-            }
         float best = -INFINITY, total = 0.0f, sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < p.splits) best = fmaxf(best, ml[k].x);
+        for (int k = 0; k < p.splits; ++k)
+            best = fmaxf(best, parts[(k * rows + r) * kPartFloats + HD]);
         const float ref = best == -INFINITY ? 0.0f : best;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < p.splits) {
-                const float f = ex2(ml[k].x - ref);
-                total = fmaf(f, v[k], total);
-                sum = fmaf(f, ml[k].y, sum);
-            }
+        for (int k = 0; k < p.splits; ++k) {
+            const float* part = parts + (k * rows + r) * kPartFloats;
+            const float f = ex2(part[HD] - ref);
+            total = fmaf(f, part[e], total);
+            sum = fmaf(f, part[HD + 1], sum);
+        }
         put(r, e, total / sum);
     }
-    __syncwarp();
-    cluster_sync();  // no CTA leaves while its part is read
 }
 
 // ------------------------------------------------------------------ tiles
@@ -1290,17 +1325,20 @@ int prepare_rows(const bl_masked_attention_args& a, Launch* out) {
     p.splits = a.key_splits ? static_cast<int>(a.key_splits)
                             : static_cast<int>(std::max<uint64_t>(
                                   1, std::min<uint64_t>({8, (888 + ctas - 1) / ctas, a.tokens / 256})));
-    if (units * p.splits > 0x7FFFFFFFull)
+    if (ctas * p.splits > 0x7FFFFFFFull)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: grid too large");
     auto kern = a.qk_dtype == BL_BF16 ? rows_kernel<true> : rows_kernel<false>;
+    const size_t smem = kRowRing + (p.splits > 1 ? p.splits * std::min<uint64_t>(combos, kMaxRows) *
+                                                       kPartFloats * sizeof(float) : 0);
     BL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(kRowSmem)));
-    const dim3 grid(static_cast<unsigned>(units * p.splits), p.kv_heads);
+                                     static_cast<int>(kRowRing + 8 * kMaxRows * kPartFloats *
+                                                                     sizeof(float))));
+    const dim3 grid(static_cast<unsigned>(ctas * p.splits));
     out->op = BL_OP_MASKED_ATTENTION;
     out->run = [=](cudaStream_t s) {
         return p.splits > 1 ? launch_k_cluster(kern, grid, dim3(32 * kRowWarps),
-                                               dim3(p.splits, 1, 1), kRowSmem, s, p)
-                            : launch_k(kern, grid, dim3(32 * kRowWarps), kRowSmem, s, p);
+                                               dim3(p.splits, 1, 1), smem, s, p)
+                            : launch_k(kern, grid, dim3(32 * kRowWarps), smem, s, p);
     };
     return BL_OK;
 }
