@@ -510,12 +510,13 @@ int prepare_rope(const bl_rope_args& a, Launch* out) {
     p.out = a.out, p.out_stride = static_cast<long long>(os);
     p.pos = a.positions, p.pos_stride = static_cast<long long>(ps);
     int j = 0;
+    const double log_theta = a.freqs == nullptr ? std::log(a.theta) : 0.0;
     for (uint32_t i = 0; i < a.axes; ++i)
         for (uint32_t k = 0; k < a.sections[i]; ++k, ++j) {
             const double f = a.freqs != nullptr ? a.freqs[j]
-                             : a.shared_ladder
-                                 ? std::pow(a.theta, -static_cast<double>(j) / static_cast<double>(pairs))
-                                 : std::pow(a.theta, -static_cast<double>(k) / a.sections[i]);
+                             : std::exp(-log_theta * (a.shared_ladder
+                                                          ? static_cast<double>(j) / static_cast<double>(pairs)
+                                                          : static_cast<double>(k) / a.sections[i]));
             if (!std::isfinite(f)) return fail(BL_ERR_INVALID, "rope: frequency %d is not finite", j);
             p.turn[j] = f / 3.14159265358979323846;
         }

@@ -274,13 +274,28 @@ PAIRING = {"half": 0, "adjacent": 1, "axis_half": 2}
 # A call of these is a few microseconds of work on the GPU, so the checks below
 # are written for few calls into torch each.
 
+class _Torch:
+    """What the calls below need of torch, looked up once."""
+
+    def __getattr__(self, name):  # the first use of any of them
+        import torch
+        self.code = {torch.float32: N.BL_F32, torch.float16: N.BL_F16, torch.bfloat16: N.BL_BF16}
+        self.int32, self.float32 = torch.int32, torch.float32
+        self.current_device = torch.cuda.current_device
+        self.raw_stream = torch._C._cuda_getCurrentRawStream
+        return self.__dict__[name]
+
+
+_T = _Torch()
+
+
 def _on_gpu(what, first, *tensors):
-    """Every tensor (None = not given) is on `first`'s GPU."""
-    if not first.is_cuda:
+    """Every tensor (None = not given) is on `first`'s GPU; its index."""
+    device = first.get_device()  # -1: not on a GPU
+    if device < 0 or not first.is_cuda:
         raise ValueError("%s: a CUDA tensor, not one on %s" % (what, first.device))
-    device = first.get_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != device):
+        if t is not None and t.get_device() != device:
             raise ValueError("%s: tensors on %s and %s" % (what, first.device, t.device))
 
 
@@ -293,15 +308,15 @@ def _table(what, t, dtype, count):
 
 def _launch(fn, args, tensor, stream):
     """Calls `fn` on `tensor`'s device, whichever device is current."""
-    import torch
     device = tensor.get_device()
-    if device != torch.cuda.current_device():
+    if device != _T.current_device():
+        import torch
         with torch.cuda.device(device):
-            N.check(fn(ctypes.byref(args), _stream_ptr(stream)))
-    elif stream is None:
-        N.check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device)))
+            rc = fn(ctypes.byref(args), _stream_ptr(stream))
     else:
-        N.check(fn(ctypes.byref(args), _stream_ptr(stream)))
+        rc = fn(ctypes.byref(args), _T.raw_stream(device) if stream is None else _stream_ptr(stream))
+    if rc:
+        N.check(rc)
 
 
 def pack_args(grids, *, offsets, image=None, positions=None, capacity=None, lead=0,
@@ -310,22 +325,21 @@ def pack_args(grids, *, offsets, image=None, positions=None, capacity=None, lead
     ``[images + 1]``; ``image``: int32 ``[capacity]`` or None; ``positions``:
     f32 ``[capacity][3]`` or None. ``capacity`` defaults to the rows of
     ``image`` or ``positions``."""
-    import torch
     _on_gpu("pack", grids, offsets, image, positions)
     shape = grids.shape
     if len(shape) != 2 or shape[1] != 3:
         raise ValueError("pack: grids are [images][3], not %s" % (tuple(shape),))
     n = shape[0]
-    _table("pack: grids", grids, torch.int32, 3 * n)
-    _table("pack: offsets", offsets, torch.int32, n + 1)
+    _table("pack: grids", grids, _T.int32, 3 * n)
+    _table("pack: offsets", offsets, _T.int32, n + 1)
     if capacity is None:
         if image is None and positions is None:
             raise ValueError("pack: a capacity, an image map or positions")
         capacity = (image if image is not None else positions).shape[0]
     if image is not None:
-        _table("pack: image", image, torch.int32, capacity)
+        _table("pack: image", image, _T.int32, capacity)
     if positions is not None:
-        _table("pack: positions", positions, torch.float32, 3 * capacity)
+        _table("pack: positions", positions, _T.float32, 3 * capacity)
         if positions.dim() != 2 or positions.shape[1] != 3:
             raise ValueError("pack: positions are [capacity][3], not %s" % (tuple(positions.shape),))
     if not 0 <= lead < 2 ** 31 or not 0 <= capacity < 2 ** 31:
@@ -377,20 +391,20 @@ def rope_args(x, positions, *, sections, theta=100.0, freqs=None, shared=False, 
             raise ValueError("rope: the values of a row's heads are neighbours")
         strides.append(st[0] if rows > 1 else 0)
     p_shape, p_stride = positions.shape, positions.stride()
-    if not 1 <= axes <= 3 or positions.dtype is not torch.float32 or len(p_shape) != 2 or \
+    if not 1 <= axes <= 3 or positions.dtype is not _T.float32 or len(p_shape) != 2 or \
             p_shape[0] < rows or p_shape[1] < axes or (axes > 1 and p_stride[1] != 1):
         raise ValueError("rope: positions %s of %s for %d rows and %d axes (1 to 3)"
                          % (tuple(p_shape), positions.dtype, rows, axes))
     if min(sections) < 1:
         raise ValueError("rope: sections %s" % (tuple(sections),))
     if dtype is None:
-        if not x.dtype.is_floating_point:
+        code = _T.code.get(x.dtype)
+        if code is None:
             raise ValueError("rope: the dtype of a %s container" % x.dtype)
-        code = _dt(x)
     else:
         code = _TD[dtype]
         if x.element_size() != (4 if dtype == "f32" else 2) or (
-                x.dtype.is_floating_point and _dt(x) != code):
+                x.dtype.is_floating_point and _T.code.get(x.dtype) != code):
             raise ValueError("rope: %s values in a tensor of %s" % (dtype, x.dtype))
     a = N.RopeArgs(rows, heads, head_dim, axes, tuple(sections), PAIRING[pairing],
                    1 if shared else 0, 1 if inverse else 0, code, theta, None, x.data_ptr(),
@@ -427,7 +441,6 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
     ``[batch]``) of each in use. ``out``: ``[rows][heads * 64]``. ``prefix``:
     int32 ``[batch]``; ``slopes``: f32 ``[heads]``; ``positions``: f32
     ``[rows][1 to 3 axes]``."""
-    import torch
     _on_gpu("masked attention", qkv, out, offsets, lengths, prefix, slopes, positions)
     kv = heads if kv_heads is None else kv_heads
     shape, st = qkv.shape, qkv.stride()
@@ -448,7 +461,7 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
     if offsets is not None:
         if batch is None:
             batch = offsets.numel() - 1
-        _table("masked attention: offsets", offsets, torch.int32, batch + 1)
+        _table("masked attention: offsets", offsets, _T.int32, batch + 1)
         tokens = rows
     else:
         if batch is None:
@@ -457,15 +470,15 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
             raise ValueError("masked attention: %d rows in %d equal parts" % (rows, batch))
         tokens = rows // batch
     if lengths is not None:
-        _table("masked attention: lengths", lengths, torch.int32, batch)
+        _table("masked attention: lengths", lengths, _T.int32, batch)
     if prefix is not None:
-        _table("masked attention: prefix", prefix, torch.int32, batch)
+        _table("masked attention: prefix", prefix, _T.int32, batch)
     if slopes is not None:
-        _table("masked attention: slopes", slopes, torch.float32, heads)
+        _table("masked attention: slopes", slopes, _T.float32, heads)
     axes = pos_stride = 0
     if positions is not None:
         p_shape, p_st = positions.shape, positions.stride()
-        if positions.dtype is not torch.float32 or len(p_shape) != 2 or p_shape[0] < rows or \
+        if positions.dtype is not _T.float32 or len(p_shape) != 2 or p_shape[0] < rows or \
                 not 1 <= p_shape[1] <= 3 or (p_shape[1] > 1 and p_st[1] != 1):
             raise ValueError("masked attention: positions are f32 [rows][1 to 3], not %s of %s"
                              % (tuple(p_shape), positions.dtype))
@@ -476,7 +489,7 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
     return N.MaskedAttentionArgs(
         batch, tokens, heads, kv, 64, min(last_rows, 2 ** 31 - 1),
         0.125 if scale is None else scale, cap or 0.0, MASK[mask], _TD[qk_dtype], N.BL_F16,
-        _dt(out) if out_dtype is None else _TD[out_dtype], qkv.data_ptr(), st[0] if many else 0,
+        _T.code[out.dtype] if out_dtype is None else _TD[out_dtype], qkv.data_ptr(), st[0] if many else 0,
         out.data_ptr(), o_st[0] if many else 0, None if offsets is None else offsets.data_ptr(),
         None if lengths is None else lengths.data_ptr(),
         None if prefix is None else prefix.data_ptr(),
@@ -491,8 +504,8 @@ def masked_attention(qkv, *, heads, out=None, out_dtype=None, stream=None, **kw)
     ``out`` a zero-filled ``[rows][heads * 64]`` of ``out_dtype`` (default
     "f16") is made on the stream; rows that are not computed are left as they
     were."""
-    import torch
     if out is None:
+        import torch
         tdt = {"f32": torch.float32, "f16": torch.float16,
                "bf16": torch.bfloat16}[out_dtype or "f16"]
         s = torch.cuda.ExternalStream(stream, device=qkv.device) if isinstance(stream, int) else stream
@@ -500,7 +513,7 @@ def masked_attention(qkv, *, heads, out=None, out_dtype=None, stream=None, **kw)
             out = torch.zeros((qkv.shape[0], heads * 64), dtype=tdt, device=qkv.device)
         out_dtype = None
     elif out.dtype.is_floating_point:
-        if out_dtype is not None and _dt(out) != _TD[out_dtype]:
+        if out_dtype is not None and _T.code.get(out.dtype) != _TD[out_dtype]:
             raise ValueError("masked attention: out is %s, not %s" % (out.dtype, out_dtype))
         out_dtype = None
     a = masked_attention_args(qkv, heads=heads, out=out, out_dtype=out_dtype, **kw)
