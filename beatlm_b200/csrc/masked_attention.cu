@@ -712,8 +712,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     if (warp == 1) {
         tmem_alloc(smem_u32(&tail->tmem_base), kTmemCols);
         tmem_relinquish();
+        // Only now may the next kernel's CTAs come beside this one (a trigger
+        // counts once a CTA, whoever gives it): before it, one of them could
+        // take the columns and wait for this kernel's end.
+        pdl_trigger();
     }
-    pdl_trigger();
     pdl_wait();
     if (warp == 0) {
         __syncwarp();
