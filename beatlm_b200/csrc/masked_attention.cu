@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "host.h"
 
@@ -20,11 +21,20 @@ namespace masked {
 constexpr int HD = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// What capping a score needs, made once on the host.
+struct Capping {
+    float unit;   // raw score -> u = s / cap
+    float c[4];   // the coefficients of tanh's series for raw scores, in log2 units
+    float twice;  // raw score -> 2 u in log2 units
+    float cap2;   // cap in log2 units
+};
+
 struct Params {
     int batch, tokens;
     int heads, kv_heads, group;  // group = heads / kv_heads
     int last_rows;
     float scale, cap;
+    Capping capping;
     int mask;
     const uint16_t* qkv;
     long long row;      // elements between rows of qkv
@@ -70,10 +80,7 @@ __device__ __forceinline__ int visible(const Params& p, const Span& q, int i) {
     return p.mask == BL_MASK_NONE ? q.len : max(i + 1, q.prefix);
 }
 
-// Scores are kept in log2 units. A capped one, cap tanh(s / cap), is formed as
-// cap - 2 cap / (1 + e^(2 s / cap)): an absolute error of a few 2^-23 cap,
-// which is what an exponent needs, from two approximate functions; it goes to
-// +-cap at the ends without a branch.
+// Scores are kept in log2 units.
 __device__ __forceinline__ float rcp_approx(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -83,6 +90,43 @@ __device__ __forceinline__ float sqrt_approx(float x) {
     float y;
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ unsigned long long both(float v) { return f2pack(v, v); }
+
+// cap tanh(s / cap) of raw scores, in log2 units. Up to |u| = |s / cap| =
+// kSmallTanh by the odd series through u^7 on the FMA units (the first term
+// left out is below 4 10^-7 of the value there), as s times a cubic in s^2.
+// Beyond it as cap - 2 cap / (1 + e^(2 u)), from two approximate functions: an
+// absolute error of a few 2^-23 cap, so a few 2^-21 of the value, for any cap;
+// it goes to +-cap at the ends without a branch. Where the whole tile of a warp
+// is below the limit (`small`) the series alone spares the unit that the
+// exponentials need two of its three functions a score.
+constexpr float kSmallTanh = 0.25f;
+__device__ __forceinline__ float capped_far(float s, const Capping& k) {
+    return fmaf(rcp_approx(1.0f + ex2(s * k.twice)), -2.0f * k.cap2, k.cap2);
+}
+__device__ __forceinline__ unsigned long long capped_small2(unsigned long long s, const Capping& k) {
+    const unsigned long long z = fmul2(s, s);
+    unsigned long long c = ffma2(z, both(k.c[3]), both(k.c[2]));
+    c = ffma2(z, c, both(k.c[1]));
+    c = ffma2(z, c, both(k.c[0]));
+    return fmul2(s, c);
+}
+template <bool kSmall>
+__device__ __forceinline__ unsigned long long capped2(unsigned long long s, const Capping& k) {
+    const unsigned long long near = capped_small2(s, k);
+    if (kSmall) return near;
+    float a, b, x, y;
+    f2unpack(s, a, b);
+    f2unpack(near, x, y);
+    return f2pack(fabsf(a * k.unit) > kSmallTanh ? capped_far(a, k) : x,
+                  fabsf(b * k.unit) > kSmallTanh ? capped_far(b, k) : y);
+}
+__device__ __forceinline__ float capped(float s, const Capping& k) {
+    float x, y;
+    f2unpack(capped2<false>(both(s), k), x, y);
+    return x;
 }
 
 // ------------------------------------------------------------------ few rows
@@ -230,8 +274,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
         for (int e = 0; e < 4; ++e) o[d][e] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     const bool capped_scores = p.cap > 0.0f;
-    const float in = capped_scores ? 2.0f * p.scale / p.cap * kLog2e : p.scale * kLog2e;
-    const float cap2 = p.cap * kLog2e;
+    const float in = p.scale * kLog2e;
+    const Capping& cap = p.capping;
 
     int stage = 0;
     for (int tile = first + warp; tile < last; tile += kRowWarps) {
@@ -267,12 +311,22 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[t][e] = f(s[t][e], e >> 1, 8 * t + (e & 1));
         };
-        if (capped_scores)
-            each([&](float x, int, int) {
-                return fmaf(rcp_approx(1.0f + ex2(x * in)), -2.0f * cap2, cap2);
-            });
-        else
+        if (capped_scores) {
+            float far = 0.0f;
+            each([&](float x, int, int) { far = fmaxf(far, fabsf(x)); return x; });
+            auto cap_all = [&](auto small) {
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2)
+                        f2unpack(capped2<decltype(small)::value>(f2pack(s[t][e], s[t][e + 1]), cap),
+                                 s[t][e], s[t][e + 1]);
+            };
+            if (__any_sync(kFull, far * cap.unit > kSmallTanh)) cap_all(std::false_type{});
+            else cap_all(std::true_type{});
+        } else {
             each([&](float x, int, int) { return x * in; });
+        }
         const int own = base + 2 * quad;  // this lane's first key
         if (p.slopes != nullptr) {
             if (p.pos == nullptr) {
@@ -605,42 +659,6 @@ __device__ __forceinline__ void store8(void* out, long long at, int dt, const fl
     }
 }
 
-// cap tanh(s / cap) of two raw scores in log2 units. Where every |u| = |s / cap|
-// of the warp's tile is at most kSmallTanh, by the odd series through u^7 on
-// the FMA units (the first term left out is below 4 10^-7 of the value there),
-// as s times a cubic in s^2: that spares the unit that the exponentials need
-// two of its three functions a score. Otherwise by those.
-constexpr float kSmallTanh = 0.25f;
-struct Capping {
-    float unit;   // raw score -> u
-    float c[4];   // the series' coefficients for raw scores, in log2 units
-    float twice;  // raw score -> 2 u in log2 units
-    float cap2;   // cap in log2 units
-    __device__ explicit Capping(const Params& p)
-        : unit(p.scale / p.cap), twice(2.0f * unit * kLog2e), cap2(p.cap * kLog2e) {
-        const float v = unit * unit;
-        c[0] = p.scale * kLog2e;
-        c[1] = c[0] * v * (-1.0f / 3.0f);
-        c[2] = c[0] * v * v * (2.0f / 15.0f);
-        c[3] = c[0] * v * v * v * (-17.0f / 315.0f);
-    }
-};
-__device__ __forceinline__ unsigned long long both(float v) { return f2pack(v, v); }
-template <bool kSmall>
-__device__ __forceinline__ unsigned long long capped2(unsigned long long s, const Capping& k) {
-    if (kSmall) {
-        const unsigned long long z = fmul2(s, s);
-        unsigned long long c = ffma2(z, both(k.c[3]), both(k.c[2]));
-        c = ffma2(z, c, both(k.c[1]));
-        c = ffma2(z, c, both(k.c[0]));
-        return fmul2(s, c);
-    }
-    float a, b;
-    f2unpack(s, a, b);
-    a = fmaf(rcp_approx(1.0f + ex2(a * k.twice)), -2.0f * k.cap2, k.cap2);
-    b = fmaf(rcp_approx(1.0f + ex2(b * k.twice)), -2.0f * k.cap2, k.cap2);
-    return f2pack(a, b);
-}
 // 32 raw scores capped in place. (A branch around each loop: inside it the two
 // forms would both be computed.)
 __device__ __forceinline__ void cap32(uint32_t (&s)[32], const Capping& k, bool small) {
@@ -923,7 +941,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         constexpr bool kCapOnly = kCap && kBias == BIAS_NONE;
         // raw scores to log2 units; kPlain does it in the exponent's FMA
         const float in = p.scale * kLog2e;
-        const Capping cap(p);  // (read under kCap alone)
+        const Capping& cap = p.capping;
         const float slope2 = kBias != BIAS_NONE ? p.slopes[head] * kLog2e : 0.0f;
         constexpr int kAxes = kBias == BIAS_SPACE ? 3 : 2;
         unsigned long long qp2[kAxes];  // this row's place, twice
@@ -1052,8 +1070,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             if (linear) m_row = fmaf(m_row, in, lean);
             // (capping keeps the order: the largest capped score is the capped
             // largest)
-            if (kCapOnly && m_row != -INFINITY)
-                m_row = fmaf(rcp_approx(1.0f + ex2(m_row * cap.twice)), -2.0f * cap.cap2, cap.cap2);
+            if (kCapOnly && m_row != -INFINITY) m_row = capped(m_row, cap);
             // R(i) from R(i - 1), the other stream's, and this tile's maximum
             float prev = -INFINITY;
             if (i > 0) {
@@ -1265,6 +1282,8 @@ int validate(const bl_masked_attention_args& a) {
         return fail(BL_ERR_INVALID, "masked attention: scale must be finite and positive");
     if (!(a.cap >= 0.0f) || !std::isfinite(a.cap))
         return fail(BL_ERR_INVALID, "masked attention: cap must be finite, 0 for none");
+    if (a.cap > 0.0f && static_cast<double>(a.scale) > 1e6 * a.cap)  // the series' coefficients
+        return fail(BL_ERR_UNSUPPORTED, "masked attention: cap below a millionth of the scale");
     if (a.mask < BL_MASK_NONE || a.mask > BL_MASK_PREFIX)
         return fail(BL_ERR_INVALID, "masked attention: mask %d", a.mask);
     if ((a.mask == BL_MASK_PREFIX) != (a.prefix != nullptr))
@@ -1305,6 +1324,15 @@ Params params_of(const bl_masked_attention_args& a) {
     p.group = static_cast<int>(a.heads / kv);
     p.last_rows = static_cast<int>(std::min(a.last_rows, a.tokens));
     p.scale = a.scale, p.cap = a.cap, p.mask = a.mask;
+    if (a.cap > 0.0f) {
+        const double unit = static_cast<double>(a.scale) / a.cap, v = unit * unit;
+        const double log2e = 1.4426950408889634;
+        const double c[4] = {1.0, -v / 3.0, v * v * (2.0 / 15.0), -v * v * v * (17.0 / 315.0)};
+        for (int i = 0; i < 4; ++i) p.capping.c[i] = static_cast<float>(a.scale * log2e * c[i]);
+        p.capping.unit = static_cast<float>(unit);
+        p.capping.twice = static_cast<float>(2.0 * unit * log2e);
+        p.capping.cap2 = static_cast<float>(a.cap * log2e);
+    }
     p.qkv = static_cast<const uint16_t*>(a.qkv);
     p.row = static_cast<long long>(a.qkv_row_stride ? a.qkv_row_stride
                                                     : (1ull * a.heads + 2ull * kv) * HD);

@@ -603,8 +603,8 @@ int bl_rope(const bl_rope_args* args, void* stream);
  * infinite included, never reach a result; within a sequence a value that is
  * not finite may reach every row of it.
  *
- * Scores, statistics and sums are f32; with more than a few query rows per K/V
- * head the probabilities are rounded to f16 for the tensor cores (as in
+ * Scores, statistics and sums are f32 (a capped score within some 2^-21 of its
+ * value); the probabilities are rounded to f16 for the tensor cores (as in
  * bl_attention). key_splits: how many CTAs share a tile's keys (a cluster,
  * combined on chip): 0 = automatic, at most 8. head_dim must be 64; qkv and out
  * 16-byte aligned with strides of 16-byte multiples. Enqueues on `stream`;
@@ -616,7 +616,7 @@ typedef struct bl_masked_attention_args {
     uint32_t heads, kv_heads, head_dim;
     uint32_t last_rows;
     float scale;
-    float cap;               /* 0 = none */
+    float cap;               /* 0 = none, else at least 1e-6 scale */
     int32_t mask;            /* BL_MASK_* */
     int32_t qk_dtype;
     int32_t v_dtype;         /* BL_F16 */

@@ -302,6 +302,27 @@ def test_capped_scores(cap, std, mask):
     Case([150, 33], seed=9, std=std).both(cap=cap, mask=mask)
 
 
+@pytest.mark.parametrize("last", [0, 1])
+@pytest.mark.parametrize("cap", [1e6, 1e12, 1e30])
+def test_a_cap_far_above_the_scores_is_none(cap, last):
+    # cap tanh(s / cap) is s less s^3 / (3 cap^2), below 1e-8 here: held to the uncapped bound
+    c = Case([150, 33], heads=2, seed=19)
+    c.check(c.run(cap=cap, last_rows=last), last_rows=last)
+
+
+@pytest.mark.parametrize("last", [1, 40])
+def test_a_capped_tile_with_one_score_far_below(last):
+    """Keys near -cap / 2 beside ordinary ones, which keep their own precision."""
+    import torch
+    c = Case([200], heads=1, qk="f16", seed=23)
+    for j, by in ((5, 6000.0), (70, 6250.0), (140, 6500.0)):
+        c.qkv[j, 1] = (c.qkv[199, 0].view(torch.float16) * -by).view(torch.int16)
+    c.k = c.qkv.view(torch.float16).double().cpu().numpy()[:, 1:2]
+    # (the keys near -cap / 2 have no weight in the last row, those of thousands all of it in
+    # the others, capped or not)
+    c.check(c.run(cap=1e5, last_rows=last), last_rows=last)
+
+
 @pytest.mark.parametrize("axes", [0, 1, 2, 3])
 @pytest.mark.parametrize("cap", [None, 20.0])
 def test_distance_bias(axes, cap):

@@ -80,7 +80,7 @@ def _attn(**kw):
     (dict(qk_dtype=N.BL_F32), "Q/K dtype"), (dict(v_dtype=N.BL_BF16), "V dtype"),
     (dict(out_dtype=7), "out dtype"), (dict(scale=0.0), "scale"),
     (dict(scale=float("nan")), "scale"), (dict(cap=-1.0), "cap"), (dict(cap=float("inf")), "cap"),
-    (dict(cap=float("nan")), "cap"), (dict(mask=3), "mask 3"), (dict(mask=2), "prefix"),
+    (dict(cap=float("nan")), "cap"), (dict(scale=0.125, cap=1e-8), "millionth"), (dict(mask=3), "mask 3"), (dict(mask=2), "prefix"),
     (dict(prefix=4 * A), "prefix"), (dict(positions=4 * A, pos_axes=2), "slopes"),
     (dict(positions=4 * A, slopes=5 * A), "position axes"),
     (dict(positions=4 * A, slopes=5 * A, pos_axes=4), "position axes"),
