@@ -875,7 +875,7 @@ class PackedEncoder:
         self.x = zeros((capacity, cfg.dim), torch.float32)
         self.xn = zeros((capacity, cfg.dim), td)
         self.qkv = zeros((capacity, 3 * cfg.dim), torch.int16)
-        # (rows behind the last image are never written: they stay zero)
+        # (rows behind the last image keep what they held: no row of an image reads them)
         self.o = zeros((capacity, cfg.dim), td)
         self.h = zeros((capacity, cfg.mlp), td)
         self.out = zeros((capacity, cfg.dim), torch.float32)

@@ -306,6 +306,14 @@ def _table(what, t, dtype, count):
                          % (what, count, dtype, tuple(t.shape), t.dtype))
 
 
+def _row_stride(what, stride, rows):
+    """The row stride an argument struct takes, where 0 says "side by side": so
+    rows that are all the same memory (an expanded tensor) are refused."""
+    if rows > 1 and stride == 0:
+        raise ValueError("%s: an expanded tensor, whose rows are one" % what)
+    return stride if rows > 1 else 0
+
+
 def _launch(fn, args, tensor, stream):
     """Calls `fn` on `tensor`'s device, whichever device is current."""
     device = tensor.get_device()
@@ -389,7 +397,7 @@ def rope_args(x, positions, *, sections, theta=100.0, freqs=None, shared=False, 
         if rows and (st[-1] != 1 and head_dim > 1
                      or len(have) == 3 and heads > 1 and st[1] != head_dim):
             raise ValueError("rope: the values of a row's heads are neighbours")
-        strides.append(st[0] if rows > 1 else 0)
+        strides.append(_row_stride("rope", st[0], rows))
     p_shape, p_stride = positions.shape, positions.stride()
     if not 1 <= axes <= 3 or positions.dtype is not _T.float32 or len(p_shape) != 2 or \
             p_shape[0] < rows or p_shape[1] < axes or (axes > 1 and p_stride[1] != 1):
@@ -408,7 +416,7 @@ def rope_args(x, positions, *, sections, theta=100.0, freqs=None, shared=False, 
             raise ValueError("rope: %s values in a tensor of %s" % (dtype, x.dtype))
     a = N.RopeArgs(rows, heads, head_dim, axes, tuple(sections), PAIRING[pairing],
                    1 if shared else 0, 1 if inverse else 0, code, theta, None, x.data_ptr(),
-                   strides[0], positions.data_ptr(), p_stride[0] if rows > 1 else 0,
+                   strides[0], positions.data_ptr(), _row_stride("rope: positions", p_stride[0], rows),
                    out.data_ptr(), strides[-1])
     if freqs is not None:
         if len(freqs) != sum(sections):
@@ -482,15 +490,15 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
                 not 1 <= p_shape[1] <= 3 or (p_shape[1] > 1 and p_st[1] != 1):
             raise ValueError("masked attention: positions are f32 [rows][1 to 3], not %s of %s"
                              % (tuple(p_shape), positions.dtype))
-        axes, pos_stride = p_shape[1], p_st[0] if rows > 1 else 0
+        axes, pos_stride = p_shape[1], _row_stride("masked attention: positions", p_st[0], rows)
     if last_rows < 0 or (cap is not None and not cap > 0):
         raise ValueError("masked attention: last_rows %s, cap %s" % (last_rows, cap))
-    many = rows > 1
     return N.MaskedAttentionArgs(
         batch, tokens, heads, kv, 64, min(last_rows, 2 ** 31 - 1),
         0.125 if scale is None else scale, cap or 0.0, MASK[mask], _TD[qk_dtype], N.BL_F16,
-        _T.code[out.dtype] if out_dtype is None else _TD[out_dtype], qkv.data_ptr(), st[0] if many else 0,
-        out.data_ptr(), o_st[0] if many else 0, None if offsets is None else offsets.data_ptr(),
+        _T.code[out.dtype] if out_dtype is None else _TD[out_dtype], qkv.data_ptr(),
+        _row_stride("masked attention: qkv", st[0], rows), out.data_ptr(),
+        _row_stride("masked attention: out", o_st[0], rows), None if offsets is None else offsets.data_ptr(),
         None if lengths is None else lengths.data_ptr(),
         None if prefix is None else prefix.data_ptr(),
         None if slopes is None else slopes.data_ptr(),

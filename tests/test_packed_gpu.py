@@ -54,6 +54,22 @@ def test_pack_of_many_images(images):
     assert np.array_equal(off, woff) and np.array_equal(img, wimg) and np.array_equal(pos, wpos)
 
 
+@pytest.mark.parametrize("normalized", [False, True])
+@pytest.mark.parametrize("shape", [(1, 2100, 2003), (3, 1, 1400001), (1, 1, 2 ** 22 + 5)])
+def test_pack_of_more_rows_than_24_bits_hold_exactly(shape, normalized):
+    """Row numbers and sides past 2^22, where places leave the f32 path."""
+    import torch
+    t, h, w = shape
+    rows = t * h * w
+    off, img, pos = _pack([shape], rows, 0, normalized)
+    r = torch.arange(rows)
+    c = torch.stack([r // (h * w), r // w % h, r % w], 1).double()
+    n = torch.tensor(shape).double()
+    want = ((2 * c + 1 - n) / n if normalized else c).numpy()
+    assert np.all(np.abs(pos - want) <= np.abs(want) * ref.EPS["f32"])  # one division
+    assert (img == 0).all() and list(off) == [0, rows]
+
+
 @pytest.mark.parametrize("grids,capacity", [
     ([(1, 4, 4), (1, 4, 4), (1, 4, 4)], 20), ([(1, 5, 5)], 7),
     ([(2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1), (1, 2, 2)], 40),
@@ -411,6 +427,26 @@ def test_offsets_and_lengths_that_point_outside_are_clamped():
     p.kw["lengths"] = torch.tensor([-3, 64], dtype=torch.int32, device="cuda")
     out = p.run().float().cpu().numpy()
     assert np.all(out[:64] == 7.0) and np.all(out[64:] != 7.0)
+
+
+def test_expanded_tensors_are_refused():
+    """Their row stride, 0, would say "side by side" and reach behind them."""
+    import torch
+    from beatlm_b200 import ops
+    one = lambda *shape: torch.zeros(shape, device="cuda").expand(4, *shape[1:])  # noqa: E731
+    x, pos, out = (torch.zeros(s, device="cuda") for s in ((4, 1, 64), (4, 2), (4, 64)))
+    for args in ((one(1, 1, 64), pos), (x, one(1, 2))):
+        with pytest.raises(ValueError, match="expanded"):
+            ops.rope(*args, sections=(16, 16))
+    with pytest.raises(ValueError, match="expanded"):
+        ops.rope(x, pos, sections=(16, 16), out=one(1, 1, 64))
+    qkv, slopes = torch.zeros((4, 3, 64), device="cuda").half(), torch.ones(1, device="cuda")
+    for q, kw in ((one(1, 3, 64).half()[:1].expand(4, 3, 64), {}), (qkv, dict(out=one(1, 64))),
+                  (qkv, dict(slopes=slopes, positions=one(1, 2)))):
+        with pytest.raises(ValueError, match="expanded"):
+            ops.masked_attention(q, heads=1, **{"out": out, **kw})
+    # one row has no stride to speak of
+    assert torch.equal(ops.rope(x[:1].expand(1, 1, 64), pos[:1], sections=(16, 16)), x[:1])
 
 
 # ------------------------------------------------------------------ as they are used
