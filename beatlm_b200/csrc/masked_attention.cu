@@ -132,18 +132,20 @@ __device__ __forceinline__ float capped(float s, const Capping& k) {
 // ------------------------------------------------------------------ few rows
 //
 // The newest rows of a stream: up to 16 query rows of one K/V head (rows and
-// heads of its group alike), for which the keys' bytes are what counts. Each
-// of a CTA's four warps walks its own 32-key tiles of one split of the keys,
-// with two tiles on their way to a shared-memory ring of its own (16 KB a warp
-// in flight; no barrier between warps). 16 rows are the
-// smallest tile of the warp-level tensor instruction (m16n8k16), which takes
-// S = Q K^T and O += P V of 16 keys in 16 instructions, so the arithmetic stays
-// below the bytes: on the FMA units one row alone cost 400 instructions
-// for 16 keys. Scores, maxima, sums and O are f32, P is rounded to f16 (it is at most
-// 1: the running maximum is exact here). Warps
-// are merged once at the end; the CTAs of a cluster send their rows' parts into
-// the first one's shared memory and leave, and that adds them in rank order.
-// MEASURED_TOKEN
+// heads of its group alike), for which the keys' bytes are what counts. Each of
+// a CTA's four warps walks its own 32-key tiles of one split of the keys, one
+// tile ahead of the one it works on (8 KB each, in a shared-memory ring of the
+// warp's own, so no barrier between warps). 16 rows are the smallest tile of the
+// warp-level tensor instruction (m16n8k16), which takes S = Q K^T and O += P V
+// of 16 keys in 16 instructions, so the arithmetic stays below the bytes: on the
+// FMA units one row alone cost 400 instructions for 16 keys. Scores, maxima,
+// sums and O are f32, P is rounded to f16 for the product (it is at most 1: the
+// running maximum is exact here), which costs 2^-11 of each at most. Warps are
+// merged once at the end; the CTAs of a cluster send their rows' parts into the
+// first one's shared memory and leave, and that adds them in rank order.
+// 16 streams of up to 8192 rows, 16 heads over 8 K/V heads (155 MB): 33.3 us,
+// 71% of a copy's rate (on the FMA units 86.5). Three stages take 41.0 (fewer
+// CTAs an SM), 16-key tiles with four 39.5.
 constexpr int kRowWarps = 4;
 constexpr int kRowTile = 32;    // keys of a tile
 constexpr int kRowStages = 2;
@@ -493,6 +495,12 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
 // and for the exponentials (a 32-column load takes 17 clocks of a warp
 // scheduler's TMEM port, 32 exponentials 256), which leaves it within the 96
 // registers that ten warps and two CTAs allow.
+// One sequence of 10960 rows, 16 heads: 632 us, 778 TFLOP/s; the exponentials'
+// unit is busy for 78% of a step (776 clocks of an SM for 128 x 64 scores, 512
+// at its rate; the rest is the softmax threads' way from S to the running
+// maximum, which the four of a scheduler cover in part). Making an eighth to a
+// third of the exponentials by a polynomial on the FMA units lengthens that way
+// and takes 645 to 670 us. A CTA's start and end cost 9000 clocks beside its steps.
 // Tiles start at their sequence's first row, so a key tile holds keys of one
 // sequence, and past its end only rows that no query sees: their scores are
 // replaced by -inf and their V rows zeroed in shared memory before the
@@ -1352,7 +1360,8 @@ int prepare_rows(const bl_masked_attention_args& a, Launch* out) {
     p.chunks = static_cast<int>((combos + kMaxRows - 1) / kMaxRows);
     const uint64_t units = 1ull * p.chunks * a.batch, ctas = units * p.kv_heads;
     // Splits: enough CTAs for three an SM twice over (sequences differ in
-    // length), each with 256 keys at least. MEASURED_SPLITS
+    // length), each with 256 keys at least. 16 streams of up to 8192 rows and
+    // 8 K/V heads: 2 splits 44.4 us, 3 35.9, 4 35.2, 6 34.3, 8 35.0.
     p.splits = a.key_splits ? static_cast<int>(a.key_splits)
                             : static_cast<int>(std::max<uint64_t>(
                                   1, std::min<uint64_t>({8, (888 + ctas - 1) / ctas, a.tokens / 256})));
