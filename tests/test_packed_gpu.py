@@ -449,6 +449,34 @@ def test_expanded_tensors_are_refused():
     assert torch.equal(ops.rope(x[:1].expand(1, 1, 64), pos[:1], sections=(16, 16)), x[:1])
 
 
+@pytest.mark.parametrize("last", [0, 1])
+def test_rows_past_32_bit_offsets(last):
+    """Rows 65536 values apart, the sequence behind 2^31 of them: rotation in
+    place, then attention, both strided."""
+    import torch
+    from beatlm_b200 import ops
+    rows, begin, stride = 33000, 32780, 65536
+    c = Case([rows - begin], heads=2, kv=1, gap=0, seed=31)
+    big = torch.empty((rows, stride), dtype=torch.int16, device="cuda")
+    out = torch.empty((rows, stride), dtype=torch.bfloat16, device="cuda")
+    qkv, o = big[:, :256], out[:, :128]
+    qkv[begin:] = c.qkv.reshape(-1, 256)
+    o.fill_(7.0)
+    pos = torch.zeros((rows, 2), device="cuda")
+    pos[begin:] = torch.rand((rows - begin, 2), device="cuda") * 40
+    ops.rope(qkv, pos, sections=(16, 16), heads=3, head_dim=64, dtype="bf16")
+    x, t = (v.reshape(-1, 4, 64)[:, :3].view(torch.bfloat16) for v in (c.qkv, qkv[begin:]))
+    _check_rope(t, x.contiguous(), pos[begin:], (16, 16), "bf16", theta=100.0, pairing="half",
+                inverse=False)
+    offsets = torch.tensor([begin, rows], dtype=torch.int32, device="cuda")
+    ops.masked_attention(qkv, heads=2, kv_heads=1, qk_dtype="bf16", offsets=offsets, mask="causal",
+                         last_rows=last, out=o)
+    assert torch.all(o[:begin] == 7.0)
+    t = t.double().cpu().numpy()
+    c.q, c.k = t[:, :2], t[:, 2:]
+    c.check(o[begin:].contiguous(), mask="causal", last_rows=last)
+
+
 # ------------------------------------------------------------------ as they are used
 
 def test_a_recorded_launch_follows_its_lengths():
