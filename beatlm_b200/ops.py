@@ -368,6 +368,20 @@ def pack(grids, *, offsets, image=None, positions=None, capacity=None, lead=0, n
     return offsets
 
 
+def _rope_stride(t, shape, dtype, rows, heads, head_dim):
+    """The row stride of a tensor of rope's, x or out, once it is the right one."""
+    st = t.stride()
+    if t.dtype is not dtype or len(shape) not in (2, 3) or shape[0] != rows or (
+            shape[1] < heads * head_dim if len(shape) == 2
+            else shape[1] != heads or shape[2] != head_dim):
+        raise ValueError("rope: %s of %s for %d rows of %d heads of %d"
+                         % (tuple(shape), t.dtype, rows, heads, head_dim))
+    if rows and (st[-1] != 1 and head_dim > 1
+                 or len(shape) == 3 and heads > 1 and st[1] != head_dim):
+        raise ValueError("rope: the values of a row's heads are neighbours")
+    return _row_stride("rope", st[0], rows)
+
+
 def rope_args(x, positions, *, sections, theta=100.0, freqs=None, shared=False, pairing="half",
               inverse=False, heads=None, head_dim=None, dtype=None, out=None):
     """``x``: ``[rows][heads][head_dim]``, or ``[rows][width]`` with ``heads``
@@ -375,29 +389,19 @@ def rope_args(x, positions, *, sections, theta=100.0, freqs=None, shared=False, 
     takes its type from ``dtype``). ``positions``: f32 ``[rows][axes or
     more]``, the axes its first columns. ``sections``: the pairs of each axis.
     ``freqs``: the host's own radians a unit of position, one a pair."""
-    import torch
     out = x if out is None else out
     _on_gpu("rope", x, positions, out)
     shape, axes = x.shape, len(sections)
-    rows = shape[0] if shape else 0
-    if len(shape) == 3:
+    dims = len(shape)
+    rows = shape[0] if dims else 0
+    if dims == 3:
         if (heads or shape[1]) != shape[1] or (head_dim or shape[2]) != shape[2]:
             raise ValueError("rope: %s heads of %s in %s" % (heads, head_dim, tuple(shape)))
         heads, head_dim = shape[1], shape[2]
-    if len(shape) not in (2, 3) or not heads or not head_dim:
+    if dims not in (2, 3) or not heads or not head_dim:
         raise ValueError("rope: x is [rows][heads][head_dim], or [rows][width] with both given")
-    strides = []
-    for t in (x,) if out is x else (x, out):
-        have, st = t.shape, t.stride()
-        if t.dtype is not x.dtype or len(have) not in (2, 3) or have[0] != rows or \
-                (len(have) == 3 and tuple(have[1:]) != (heads, head_dim)) or \
-                (len(have) == 2 and have[1] < heads * head_dim):
-            raise ValueError("rope: %s of %s for %d rows of %d heads of %d"
-                             % (tuple(have), t.dtype, rows, heads, head_dim))
-        if rows and (st[-1] != 1 and head_dim > 1
-                     or len(have) == 3 and heads > 1 and st[1] != head_dim):
-            raise ValueError("rope: the values of a row's heads are neighbours")
-        strides.append(_row_stride("rope", st[0], rows))
+    x_stride = _rope_stride(x, shape, x.dtype, rows, heads, head_dim)
+    o_stride = x_stride if out is x else _rope_stride(out, out.shape, x.dtype, rows, heads, head_dim)
     p_shape, p_stride = positions.shape, positions.stride()
     if not 1 <= axes <= 3 or positions.dtype is not _T.float32 or len(p_shape) != 2 or \
             p_shape[0] < rows or p_shape[1] < axes or (axes > 1 and p_stride[1] != 1):
@@ -416,8 +420,8 @@ def rope_args(x, positions, *, sections, theta=100.0, freqs=None, shared=False, 
             raise ValueError("rope: %s values in a tensor of %s" % (dtype, x.dtype))
     a = N.RopeArgs(rows, heads, head_dim, axes, tuple(sections), PAIRING[pairing],
                    1 if shared else 0, 1 if inverse else 0, code, theta, None, x.data_ptr(),
-                   strides[0], positions.data_ptr(), _row_stride("rope: positions", p_stride[0], rows),
-                   out.data_ptr(), strides[-1])
+                   x_stride, positions.data_ptr(), _row_stride("rope: positions", p_stride[0], rows),
+                   out.data_ptr(), o_stride)
     if freqs is not None:
         if len(freqs) != sum(sections):
             raise ValueError("rope: %d frequencies for sections %s" % (len(freqs), tuple(sections)))
