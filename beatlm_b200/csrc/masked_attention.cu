@@ -50,6 +50,7 @@ struct Params {
     int pos_axes;
     int splits;         // CTAs of a cluster that share the keys
     int chunks;         // query chunks (or tiles) a sequence has at most
+    int ragged;         // the sequences' lengths are in device memory
     Status* status;
 };
 
@@ -572,33 +573,61 @@ __device__ __forceinline__ int side_of(const Params& p, int prefix, int q0, int 
     return k0 >= q0 + BM - 1 ? -1 : 0;
 }
 
-// The sequence (its rows, without the prefix) and tile of tile `index` of the
-// packed batch, the longest sequences' tiles first while there are at most 32
-// (a warp ranks them by their lengths); otherwise in the sequences' order, which
-// a warp walks 256 at a time, eight a lane, so that a chunk costs one round trip
-// to memory. Returns the sequence, -1 behind the last tile.
+// The sequence of tile `index` of a batch of at most 32, its rows without the
+// prefix, and the tile counted from the sequence's end, in the order of the
+// tiles' keys, most first: a warp ranks them, one sequence a lane. Without a mask
+// a sequence's tiles all have its length; under one, a tile further up has BM
+// keys less, so the tiles of one level (whole tiles of rows up to the end of
+// this one) are alike, and the level follows from how many tiles lie at or above
+// each. Returns the sequence, -1 behind the last tile.
+__device__ __forceinline__ int ranked_tile(const Params& p, int index, Span& q, int& tile) {
+    constexpr unsigned kAll = 0xFFFFFFFFu;
+    const int lane = lane_id();
+    const Span mine = span_of(p, min(lane, p.batch - 1));
+    const int len = lane < p.batch ? mine.len : 0;
+    const int tiles = lane < p.batch ? (len - mine.first + BM - 1) / BM : 0;
+    bool here;
+    if (p.mask == BL_MASK_NONE) {
+        int before = 0;  // tiles of the longer sequences
+        for (int j = 0; j < p.batch; ++j) {
+            const int other = __shfl_sync(kAll, len, j), count = __shfl_sync(kAll, tiles, j);
+            if (other > len || (other == len && j < lane)) before += count;
+        }
+        tile = index - before;
+        here = tile >= 0 && tile < tiles;
+    } else {
+        const int up = (len + BM - 1) / BM;  // the last tile's level; the others' below
+        auto above = [&](int level) {        // tiles at this level or above
+            return __reduce_add_sync(kAll, min(max(up - level + 1, 0), tiles));
+        };
+        int lo = 0, hi = __reduce_max_sync(kAll, up);  // above(lo) > index, if any is
+        if (above(0) <= index) return -1;
+        while (lo < hi) {
+            const int mid = lo + (hi - lo + 1) / 2;
+            if (above(mid) > index) lo = mid; else hi = mid - 1;
+        }
+        tile = up - lo;
+        const bool has = tile >= 0 && tile < tiles;
+        const unsigned level = __ballot_sync(kAll, has);
+        const int place = index - above(lo + 1);  // within the level
+        here = has && __popc(level & ((1u << lane) - 1)) == place;
+    }
+    const unsigned found = __ballot_sync(kAll, here);
+    if (found == 0) return -1;
+    const int owner = __ffs(found) - 1;
+    q.begin = __shfl_sync(kAll, mine.begin, owner);
+    q.len = __shfl_sync(kAll, len, owner);
+    q.first = __shfl_sync(kAll, mine.first, owner);
+    tile = __shfl_sync(kAll, tile, owner);
+    return owner;
+}
+
+// The same for a packed batch of more sequences, all their rows: in the
+// sequences' order, which a warp walks 256 at a time, eight a lane, so that a
+// chunk costs one round trip to memory.
 __device__ __forceinline__ int find_tile(const Params& p, int index, int& begin, int& len,
                                          int& tile) {
     const int lane = lane_id();
-    if (p.batch <= 32) {
-        // one sequence a lane: the tiles of the longer ones come before its own
-        const int b = min(max(p.offsets[min(lane, p.batch)], 0), p.tokens);
-        const int e = min(max(p.offsets[min(lane + 1, p.batch)], 0), p.tokens);
-        const int rows = max(e - b, 0);
-        int before = 0;
-        for (int j = 0; j < p.batch; ++j) {
-            const int other = __shfl_sync(0xFFFFFFFFu, rows, j);
-            if (other > rows || (other == rows && j < lane)) before += (other + BM - 1) / BM;
-        }
-        const bool here = index >= before && index < before + (rows + BM - 1) / BM;
-        const unsigned found = __ballot_sync(0xFFFFFFFFu, here);
-        if (found == 0) return -1;
-        const int owner = __ffs(found) - 1;
-        begin = __shfl_sync(0xFFFFFFFFu, b, owner);
-        len = __shfl_sync(0xFFFFFFFFu, rows, owner);
-        tile = __shfl_sync(0xFFFFFFFFu, index - before, owner);
-        return owner;
-    }
     int total = 0;
     for (int base = 0; base < p.batch; base += 256) {
         const int first = base + 8 * lane;
@@ -712,6 +741,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const int unit = static_cast<int>(work / static_cast<unsigned>(p.heads));
     const int head = static_cast<int>(work - static_cast<unsigned>(unit) * p.heads);
     const int kvh = head / p.group;
+    const int part_rows = (BM + p.splits - 1) / p.splits;  // a CTA's rows where a cluster joins
     constexpr unsigned kFull = 0xFFFFFFFFu;
 
     if (threadIdx.x == 0) {
@@ -748,7 +778,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         __syncwarp();
         Span q{};
         int tile = 0, rows = 0, q0 = 0, first = 0, count = 0, pivot = -1;
-        if (p.chunks > 0) {
+        if (p.batch <= 32 && p.ragged) {
+            const int seq = ranked_tile(p, unit, q, tile);
+            if (seq < 0) q.len = 0;
+            else if (p.mask == BL_MASK_PREFIX) q.prefix = min(max(p.prefix[seq], 0), q.len);
+        } else if (p.chunks > 0) {
             q = span_of(p, unit % p.batch);
             tile = unit / p.batch;
         } else {
@@ -1179,83 +1213,86 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             const float top = ok ? fmaxf(m_used, other) : -INFINITY;
             const float ref = top == -INFINITY ? 0.0f : top;
             const float sum = ok ? ex2(m_used - ref) * l + ex2(other - ref) * tail->odd_sum[row] : 0.0f;
-            const float w = p.splits == 1 ? 1.0f / sum : 1.0f;
-            const long long to = (q.begin + at) * p.out_row + head * HD;
-            float4* po = reinterpret_cast<float4*>(sK);
+            if (p.splits > 1) {
+                // the ring is free here: the last PV is complete, so every copy
+                // has landed and been read
+                __syncwarp();
+                cluster_arrive();
+                cluster_wait();
+                // the row's O, maximum and sum into its owner's ring; its vectors
+                // rotated, so that a warp's stores spread over the banks
+                const int owner = ((row + 1) * p.splits - 1) / BM;
+                const int slot = split * part_rows + row - BM * owner / p.splits;
+                const uint32_t to = dsmem_addr(smem_u32(sK) + slot * (HD * 4), owner);
+                dsmem_st2(dsmem_addr(smem_u32(sV) + slot * 8, owner), top, sum);
 #pragma unroll
-            for (int h = 0; h < HD / 16; ++h) {
-                uint32_t a[16];
+                for (int h = 0; h < HD / 16; ++h) {
+                    uint32_t a[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) a[k] = 0;
-                if (ok && n > 0) tmem_ld16(o_col + 16 * h, a);
-                tmem_wait_ld();
-                float v[16];
+                    for (int k = 0; k < 16; ++k) a[k] = 0;
+                    if (ok && n > 0) tmem_ld16(o_col + 16 * h, a);
+                    tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = w * __uint_as_float(a[k]);
-                if (p.splits == 1) {
+                    for (int k = 0; k < 4; ++k)
+                        dsmem_st4u(to + 16 * ((4 * h + k) ^ (slot & 15)),
+                                   make_uint4(a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3]));
+                }
+            } else {
+                const float w = 1.0f / sum;
+                const long long to = (q.begin + at) * p.out_row + head * HD;
+#pragma unroll
+                for (int h = 0; h < HD / 16; ++h) {
+                    uint32_t a[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) a[k] = 0;
+                    if (ok && n > 0) tmem_ld16(o_col + 16 * h, a);
+                    tmem_wait_ld();
+                    float v[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v[k] = w * __uint_as_float(a[k]);
                     if (ok && live) {
                         store8(p.out, to + 16 * h, p.out_dtype, v);
                         store8(p.out, to + 16 * h + 8, p.out_dtype, v + 8);
                     }
-                } else {
-                    // the split's O of each row into the K ring, free by now
-                    // (the last PV is complete, so every copy has landed and
-                    // been read); a row's vectors rotated so that a warp's
-                    // stores spread over the banks
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        po[row * 16 + ((4 * h + k) ^ (row & 15))] =
-                            make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
                 }
             }
-            if (p.splits > 1) reinterpret_cast<float2*>(sV)[row] = make_float2(top, sum);
         }
     }
     if (p.splits > 1) {
-        // The cluster's CTAs share out the tile's rows; each adds every
-        // split's part of its rows in rank order (the same bits in every run).
+        // The cluster's CTAs share out the tile's rows, and each has every
+        // split's part of its own sent to it (stores into its shared memory,
+        // which nobody waits for but the barrier): it adds them in rank order
+        // (the same bits in every run) and no CTA reads another's memory.
         __syncwarp();
-        fence_cluster();
+        if (warp < kSoftmaxWarp0 || warp >= kSoftmaxWarp0 + 4) {
+            cluster_arrive();
+            cluster_wait();
+        }
+        __syncwarp();
         cluster_sync();
-        const int me = static_cast<int>(cluster_rank());
+        const int me = static_cast<int>(split);
         const int r0 = BM * me / p.splits, r1 = min(BM * (me + 1) / p.splits, tail->rows);
         const long long to = (tail->span.begin + tail->q0) * p.out_row + head * HD;
-        // (the loop's bound is the warp's, so that the warp reaches the cluster
-        // barrier after it as one)
-        for (int w0 = r0 * 16 + 32 * warp; w0 < r1 * 16; w0 += kTileThreads) {
-            const int i = min(w0 + lane, r1 * 16 - 1);  // the last lanes repeat a store
-            const int row = i >> 4, k = i & 15;
-            const uint32_t at_ml = smem_u32(sV) + row * 8;
-            const uint32_t at_o = smem_u32(sK) + (row * 16 + (k ^ (row & 15))) * 16;
-            float2 ml[8];
-            float4 o[8];
-#pragma unroll
-            for (int s = 0; s < 8; ++s)  // every load on its way before the first use
-                if (s < p.splits) {
-                    ml[s] = dsmem_ld2(dsmem_addr(at_ml, s));
-                    o[s] = dsmem_ld4(dsmem_addr(at_o, s));
-                }
+        for (int i = threadIdx.x; i < (r1 - r0) * 16; i += kTileThreads) {
+            const int r = i >> 4, k = i & 15;
+            const float2* ml = reinterpret_cast<const float2*>(sV) + r;
             float top = -INFINITY;
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-                if (s < p.splits) top = fmaxf(top, ml[s].x);
+            for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[s * part_rows].x);
             const float ref = top == -INFINITY ? 0.0f : top;
             float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float sum = 0.0f;
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-                if (s < p.splits) {
-                    const float w = ex2(ml[s].x - ref);
-                    sum = fmaf(w, ml[s].y, sum);
-                    a.x = fmaf(w, o[s].x, a.x), a.y = fmaf(w, o[s].y, a.y);
-                    a.z = fmaf(w, o[s].z, a.z), a.w = fmaf(w, o[s].w, a.w);
-                }
+            for (int s = 0; s < p.splits; ++s) {
+                const int slot = s * part_rows + r;
+                const float4 o = reinterpret_cast<const float4*>(sK)[slot * 16 + (k ^ (slot & 15))];
+                const float w = ex2(ml[s * part_rows].x - ref);
+                sum = fmaf(w, ml[s * part_rows].y, sum);
+                a.x = fmaf(w, o.x, a.x), a.y = fmaf(w, o.y, a.y);
+                a.z = fmaf(w, o.z, a.z), a.w = fmaf(w, o.w, a.w);
+            }
             const float inv = 1.0f / sum;
-            store4(p.out, to + row * p.out_row + 4 * k, p.out_dtype,
+            store4(p.out, to + (r0 + r) * p.out_row + 4 * k, p.out_dtype,
                    make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
         }
-        __syncwarp();
-        cluster_sync();  // no CTA leaves while its part is read
     }
     tc_fence_before();
     __syncthreads();
@@ -1350,6 +1387,7 @@ Params params_of(const bl_masked_attention_args& a) {
     p.slopes = a.slopes, p.pos = a.positions;
     p.pos_row = static_cast<long long>(a.pos_row_stride ? a.pos_row_stride : a.pos_axes);
     p.pos_axes = static_cast<int>(a.pos_axes);
+    p.ragged = a.offsets != nullptr || a.lengths != nullptr;
     p.status = status_ptr();
     return p;
 }
@@ -1394,11 +1432,23 @@ int prepare_tiles(const bl_masked_attention_args& a, Launch* out) {
                                   : per_seq * a.batch;
     p.chunks = packed ? 0 : static_cast<int>(per_seq);
     // Split the keys while that many CTAs still run at once (two an SM) and
-    // each keeps 256 keys of an average sequence.
+    // each keeps 256 keys of an average sequence. A whole wave of unlike CTAs
+    // waits for its longest: where a mask makes them unlike, halves are better
+    // from 1536 keys on (5477 rows causal, 6 heads: 71.4 -> 47.1 us; 3 x 1800:
+    // 36.4 -> 28.3; but 3 x 1370 without a mask: 26.5 -> 28.8), and in any case
+    // where a wave is long (4096 keys: 5477 rows, 5 heads, no mask 81.4 -> 63.2;
+    // 8 heads, 344 CTAs: 106.6 -> 97.9, while 430 lose). Lengths that only the
+    // device knows count as unlike: quarters of half a wave (2 x 1370 newest rows
+    // of 5480 and 2000, 6 heads: 45.7 -> 37.7; of 5480 twice: 47.8 -> 49.1).
     const uint64_t keys = a.offsets != nullptr ? a.tokens / a.batch : a.tokens;
-    p.splits = a.key_splits ? static_cast<int>(a.key_splits)
-                            : static_cast<int>(std::max<uint64_t>(
-                                  1, std::min<uint64_t>({8, 296 / (units * p.heads), keys / 256})));
+    const uint64_t ctas = units * p.heads;
+    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>({8, 2 * kSms / ctas, keys / 256}));
+    if (splits == 1 && ctas <= 370 &&
+        keys >= (p.mask != BL_MASK_NONE && ctas <= 2 * kSms ? 1536u : 4096u))
+        splits = 2;
+    else if (splits == 2 && p.ragged && a.batch > 1 && keys >= 1536)
+        splits = 4;
+    p.splits = static_cast<int>(a.key_splits ? a.key_splits : splits);
     if (units * p.heads * p.splits > 0x7FFFFFFFull)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: grid too large");
     const uint64_t rows = a.offsets != nullptr ? a.tokens : 1ull * a.batch * a.tokens;

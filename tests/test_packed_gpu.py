@@ -381,6 +381,19 @@ def test_key_splits(splits, last):
     assert np.array_equal(c.run(**kw).float().cpu().numpy(), c.run(**kw).float().cpu().numpy())
 
 
+@pytest.mark.parametrize("batch", [2, 31, 32, 33])
+@pytest.mark.parametrize("form", ["packed", "padded"])
+@pytest.mark.parametrize("mask", [None, "causal", "prefix"])
+@pytest.mark.parametrize("last", [0, 150])
+def test_every_tile_of_a_ragged_batch_is_found(batch, form, mask, last):
+    """Tiles are ranked by their keys up to 32 sequences, walked beyond."""
+    rng = np.random.default_rng(batch + last)
+    lens = [int(v) for v in rng.integers(0, 400, batch)]
+    lens[0], lens[-1] = 385, 0
+    kw = {"prefix": [int(v) for v in rng.integers(0, 400, batch)]} if mask == "prefix" else {}
+    Case(lens, heads=1, form=form, seed=batch).both(mask=mask, last_rows=last, **kw)
+
+
 def test_padded_batch_without_lengths_and_strided_rows():
     import torch
     c = Case([96, 96, 96], heads=2, kv=1, form="padded", extra=3)
