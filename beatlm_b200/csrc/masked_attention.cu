@@ -19,6 +19,7 @@ namespace bl {
 namespace masked {
 
 constexpr int HD = 64;
+constexpr unsigned kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What capping a score needs, made once on the host.
@@ -144,9 +145,9 @@ __device__ __forceinline__ float capped(float s, const Capping& k) {
 // running maximum is exact here), which costs 2^-11 of each at most. Warps are
 // merged once at the end; the CTAs of a cluster send their rows' parts into the
 // first one's shared memory and leave, and that adds them in rank order.
-// 16 streams of up to 8192 rows, 16 heads over 8 K/V heads (155 MB): 33.3 us,
-// 71% of a copy's rate (on the FMA units 86.5). Three stages take 41.0 (fewer
-// CTAs an SM), 16-key tiles with four 39.5.
+// 16 streams of up to 8192 rows, 16 heads over 8 K/V heads (155 MB): 31.2 us,
+// 76% of a copy's rate (on the FMA units 86.5). Three stages take a fifth
+// longer (fewer CTAs an SM), 16-key tiles with four 15%.
 constexpr int kRowWarps = 4;
 constexpr int kRowTile = 32;    // keys of a tile
 constexpr int kRowStages = 2;
@@ -201,7 +202,18 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
     const int unit = static_cast<int>(work / static_cast<unsigned>(p.kv_heads));
     const int kvh = static_cast<int>(work - static_cast<unsigned>(unit) * p.kv_heads);
     const int c0 = unit % p.chunks * kMaxRows;
-    const Span q = span_of(p, unit / p.chunks);
+    // the longest streams first: their CTAs are not the last to start
+    int seq = unit / p.chunks;
+    if (p.ragged && p.batch <= 32) {
+        const int len = span_of(p, min(lane, p.batch - 1)).len;
+        int longer = lane < p.batch ? 0 : p.batch;
+        for (int j = 0; j < p.batch; ++j) {
+            const int other = __shfl_sync(kFull, len, j);
+            longer += other > len || (other == len && j < lane);
+        }
+        seq = __ffs(__ballot_sync(kFull, longer == seq && lane < p.batch)) - 1;
+    }
+    const Span q = span_of(p, seq);
     const int rows = min((q.len - q.first) * p.group - c0, kMaxRows);
     if (rows <= 0) return;  // the whole cluster leaves
     if (p.splits > 1) {
@@ -510,7 +522,6 @@ constexpr int BM = 128;
 constexpr int BN = 64;
 constexpr int STAGES = 5;  // K/V ring
 constexpr int SBUFS = 3;
-constexpr unsigned kSms = 148;
 constexpr int kTileThreads = 320;  // two CTAs of 96 registers a thread
 constexpr int kSoftmaxWarp0 = 2;
 constexpr uint32_t kQBytes = BM * HD * 2;
@@ -1397,12 +1408,15 @@ int prepare_rows(const bl_masked_attention_args& a, Launch* out) {
     const uint64_t combos = 1ull * p.last_rows * p.group;
     p.chunks = static_cast<int>((combos + kMaxRows - 1) / kMaxRows);
     const uint64_t units = 1ull * p.chunks * a.batch, ctas = units * p.kv_heads;
-    // Splits: enough CTAs for three an SM twice over (sequences differ in
-    // length), each with 256 keys at least. 16 streams of up to 8192 rows and
-    // 8 K/V heads: 2 splits 44.4 us, 3 35.9, 4 35.2, 6 34.3, 8 35.0.
-    p.splits = a.key_splits ? static_cast<int>(a.key_splits)
-                            : static_cast<int>(std::max<uint64_t>(
-                                  1, std::min<uint64_t>({8, (888 + ctas - 1) / ctas, a.tokens / 256})));
+    // Splits: as many as run at once (three CTAs an SM), each with 256 keys at
+    // least; where that leaves three or fewer and the streams are long, about 768
+    // CTAs, so that lengths that differ, and a wave that is not full, even out.
+    // 16 streams of up to 8192 rows, 8 K/V heads: 2 splits 40.5 us, 3 35.9, 4
+    // 30.4, 6 31.2, 8 35.7; of 8192 each: 45.8, 48.7, 54.7, 46.6, 49.6; of 2048
+    // each: 14.1, 12.6, 16.7, 15.8, 18.9.
+    uint64_t splits = std::min<uint64_t>({8, 3 * kSms / ctas, a.tokens / 256});
+    if (3 * kSms / ctas <= 3 && a.tokens >= 4096) splits = std::max(splits, (768 + ctas / 2) / ctas);
+    p.splits = static_cast<int>(a.key_splits ? a.key_splits : std::max<uint64_t>(1, splits));
     if (ctas * p.splits > 0x7FFFFFFFull)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: grid too large");
     auto kern = a.qk_dtype == BL_BF16 ? rows_kernel<true> : rows_kernel<false>;
