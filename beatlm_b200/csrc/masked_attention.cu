@@ -52,6 +52,7 @@ struct Params {
     int splits;         // CTAs of a cluster that share the keys
     int chunks;         // query chunks (or tiles) a sequence has at most
     int ragged;         // the sequences' lengths are in device memory
+    int mixed;          // a cluster splits the keys of long tiles alone
     Status* status;
 };
 
@@ -570,6 +571,7 @@ struct TileTail {
     int q0, rows;   // first query row within the sequence, rows of the tile (0: no work)
     int t0, n;      // its key tiles
     int pivot;      // the one with the nearest keys, of the n; -1: in rising order
+    int splits, split;  // CTAs that share the tile's keys, and which of them this is
     float ref[2][BM];      // R after the stream's last tile
     float odd_sum[BM];
 };
@@ -584,19 +586,54 @@ __device__ __forceinline__ int side_of(const Params& p, int prefix, int q0, int 
     return k0 >= q0 + BM - 1 ? -1 : 0;
 }
 
+constexpr int kLongTile = 12;  // key tiles that a tile has at least to be shared
+
 // The sequence of tile `index` of a batch of at most 32, its rows without the
 // prefix, and the tile counted from the sequence's end, in the order of the
 // tiles' keys, most first: a warp ranks them, one sequence a lane. Without a mask
 // a sequence's tiles all have its length; under one, a tile further up has BM
 // keys less, so the tiles of one level (whole tiles of rows up to the end of
 // this one) are alike, and the level follows from how many tiles lie at or above
-// each. Returns the sequence, -1 behind the last tile.
-__device__ __forceinline__ int ranked_tile(const Params& p, int index, Span& q, int& tile) {
+// each. With p.mixed a cluster shares the keys of one tile while the tile is
+// long, and its CTAs take a tile each of the shorter ones (`parts` 1). What is
+// long follows from the mean of the tiles' keys over the CTAs that run at once:
+// without a mask half as much again (parts cost a start and a join each, so a
+// split pays where the tile alone would outlast the others), under one the mean
+// (the tiles below it are many), and where tiles left whole, which start last,
+// would outlast them, half of a part of the longest.
+// Returns the sequence, -1 behind the last tile.
+__device__ __forceinline__ int ranked_tile(const Params& p, int index, Span& q, int& tile,
+                                           int& parts, int& part) {
     constexpr unsigned kAll = 0xFFFFFFFFu;
     const int lane = lane_id();
     const Span mine = span_of(p, min(lane, p.batch - 1));
     const int len = lane < p.batch ? mine.len : 0;
     const int tiles = lane < p.batch ? (len - mine.first + BM - 1) / BM : 0;
+    const int up = (len + BM - 1) / BM;  // the last tile's level; the others' below
+    auto above = [&](int level) {        // tiles at this level or above
+        return __reduce_add_sync(kAll, min(max(up - level + 1, 0), tiles));
+    };
+    if (p.mixed) {
+        // key tiles of a head's tiles (longer streams count as 2^16 levels)
+        const int most = 2 * min(up, 1 << 16), bound = min(tiles, 1 << 12);
+        const int sum = bound * (p.mask == BL_MASK_NONE ? most : max(most - bound + 1, 0));
+        const float mean = static_cast<float>(__reduce_add_sync(kAll, sum >> 5)) * 32.0f *
+                           static_cast<float>(p.heads) / (2 * kSms);
+        const float part_of = 0.5f * static_cast<float>(__reduce_max_sync(kAll, most)) / p.splits;
+        const bool wave = gridDim.x <= 2 * kSms * p.splits;  // all tiles whole would be one
+        const float from = p.splits > 2               ? part_of
+                           : p.mask == BL_MASK_NONE   ? 1.5f * mean
+                           : wave && part_of < mean   ? part_of
+                                                      : mean;
+        const int limit = max(static_cast<int>(from), kLongTile);
+        const int shared = p.mask == BL_MASK_NONE
+                               ? __reduce_add_sync(kAll, most > limit ? tiles : 0)
+                               : above(limit / 2 + 1);
+        if (index >= shared) {
+            index = shared + (index - shared) * parts + part;
+            parts = 1, part = 0;
+        }
+    }
     bool here;
     if (p.mask == BL_MASK_NONE) {
         int before = 0;  // tiles of the longer sequences
@@ -607,10 +644,6 @@ __device__ __forceinline__ int ranked_tile(const Params& p, int index, Span& q, 
         tile = index - before;
         here = tile >= 0 && tile < tiles;
     } else {
-        const int up = (len + BM - 1) / BM;  // the last tile's level; the others' below
-        auto above = [&](int level) {        // tiles at this level or above
-            return __reduce_add_sync(kAll, min(max(up - level + 1, 0), tiles));
-        };
         int lo = 0, hi = __reduce_max_sync(kAll, up);  // above(lo) > index, if any is
         if (above(0) <= index) return -1;
         while (lo < hi) {
@@ -745,14 +778,13 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     // cluster), then the heads of a tile, so that the tiles with most keys (the
     // first units) start first in every head and the last CTAs are short
     unsigned work = blockIdx.x / static_cast<unsigned>(p.splits);
-    const unsigned split = blockIdx.x - work * p.splits;
+    const int rank = static_cast<int>(blockIdx.x - work * p.splits);
     // (one CTA an SM goes out before any SM gets its second: where all fit at
     // once, the second ones come lightest first, beside the heaviest)
     if (p.splits == 1 && gridDim.x <= 2 * kSms && work >= kSms) work = gridDim.x - 1 - (work - kSms);
     const int unit = static_cast<int>(work / static_cast<unsigned>(p.heads));
     const int head = static_cast<int>(work - static_cast<unsigned>(unit) * p.heads);
     const int kvh = head / p.group;
-    const int part_rows = (BM + p.splits - 1) / p.splits;  // a CTA's rows where a cluster joins
     constexpr unsigned kFull = 0xFFFFFFFFu;
 
     if (threadIdx.x == 0) {
@@ -789,8 +821,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         __syncwarp();
         Span q{};
         int tile = 0, rows = 0, q0 = 0, first = 0, count = 0, pivot = -1;
-        if (p.batch <= 32 && p.ragged) {
-            const int seq = ranked_tile(p, unit, q, tile);
+        int parts = p.splits, part = rank;
+        if (p.batch <= 32 && (p.ragged || p.mixed)) {
+            const int seq = ranked_tile(p, unit, q, tile, parts, part);
             if (seq < 0) q.len = 0;
             else if (p.mask == BL_MASK_PREFIX) q.prefix = min(max(p.prefix[seq], 0), q.len);
         } else if (p.chunks > 0) {
@@ -810,8 +843,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             rows = min(q.len - q0, BM);
             // below 2^25 tiles and at most 8 splits: 32 bits hold the products
             const unsigned nt = (visible(p, q, q0 + rows - 1) + BN - 1) / BN;
-            first = static_cast<int>(nt * split / p.splits);
-            count = static_cast<int>(nt * (split + 1) / p.splits) - first;
+            first = static_cast<int>(nt * part / parts);
+            count = static_cast<int>(nt * (part + 1) / parts) - first;
             if (kBias != BIAS_NONE)
                 pivot = min(max((q0 + rows - 1) / BN - first, -1), count - 1);
         }
@@ -819,6 +852,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             tail->span = q;
             tail->q0 = q0, tail->rows = rows, tail->t0 = first, tail->n = count;
             tail->pivot = pivot;
+            tail->splits = parts, tail->split = part;
         }
         __syncwarp();
     }
@@ -839,11 +873,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tail->tmem_base;
-    if (tail->rows == 0) {  // no such tile (the same for every CTA of a cluster)
+    if (tail->rows == 0) {  // no such tile (for all that would share it)
         if (warp == 1) tmem_dealloc(tmem, kTmemCols);
         return;
     }
     const int t0 = tail->t0, n = tail->n;
+    const int splits = tail->splits, part_rows = (BM + splits - 1) / splits;
     // The first key of the i-th tile. With a bias of distance the nearest keys
     // come first, those before them downwards, then those behind: the largest
     // scores are then met at once, and the running maximum that O is relative
@@ -1224,7 +1259,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             const float top = ok ? fmaxf(m_used, other) : -INFINITY;
             const float ref = top == -INFINITY ? 0.0f : top;
             const float sum = ok ? ex2(m_used - ref) * l + ex2(other - ref) * tail->odd_sum[row] : 0.0f;
-            if (p.splits > 1) {
+            if (splits > 1) {
                 // the ring is free here: the last PV is complete, so every copy
                 // has landed and been read
                 __syncwarp();
@@ -1232,8 +1267,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 cluster_wait();
                 // the row's O, maximum and sum into its owner's ring; its vectors
                 // rotated, so that a warp's stores spread over the banks
-                const int owner = ((row + 1) * p.splits - 1) / BM;
-                const int slot = split * part_rows + row - BM * owner / p.splits;
+                const int owner = ((row + 1) * splits - 1) / BM;
+                const int slot = tail->split * part_rows + row - BM * owner / splits;
                 const uint32_t to = dsmem_addr(smem_u32(sK) + slot * (HD * 4), owner);
                 dsmem_st2(dsmem_addr(smem_u32(sV) + slot * 8, owner), top, sum);
 #pragma unroll
@@ -1269,7 +1304,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             }
         }
     }
-    if (p.splits > 1) {
+    if (splits > 1) {
         // The cluster's CTAs share out the tile's rows, and each has every
         // split's part of its own sent to it (stores into its shared memory,
         // which nobody waits for but the barrier): it adds them in rank order
@@ -1281,18 +1316,18 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
         __syncwarp();
         cluster_sync();
-        const int me = static_cast<int>(split);
-        const int r0 = BM * me / p.splits, r1 = min(BM * (me + 1) / p.splits, tail->rows);
+        const int me = tail->split;
+        const int r0 = BM * me / splits, r1 = min(BM * (me + 1) / splits, tail->rows);
         const long long to = (tail->span.begin + tail->q0) * p.out_row + head * HD;
         for (int i = threadIdx.x; i < (r1 - r0) * 16; i += kTileThreads) {
             const int r = i >> 4, k = i & 15;
             const float2* ml = reinterpret_cast<const float2*>(sV) + r;
             float top = -INFINITY;
-            for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[s * part_rows].x);
+            for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s * part_rows].x);
             const float ref = top == -INFINITY ? 0.0f : top;
             float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float sum = 0.0f;
-            for (int s = 0; s < p.splits; ++s) {
+            for (int s = 0; s < splits; ++s) {
                 const int slot = s * part_rows + r;
                 const float4 o = reinterpret_cast<const float4*>(sK)[slot * 16 + (k ^ (slot & 15))];
                 const float w = ex2(ml[s * part_rows].x - ref);
@@ -1445,23 +1480,27 @@ int prepare_tiles(const bl_masked_attention_args& a, Launch* out) {
     const uint64_t units = packed ? p.tokens / BM + std::min<uint64_t>(a.batch, a.tokens)
                                   : per_seq * a.batch;
     p.chunks = packed ? 0 : static_cast<int>(per_seq);
-    // Split the keys while that many CTAs still run at once (two an SM) and
-    // each keeps 256 keys of an average sequence. A whole wave of unlike CTAs
-    // waits for its longest: where a mask makes them unlike, halves are better
-    // from 1536 keys on (5477 rows causal, 6 heads: 71.4 -> 47.1 us; 3 x 1800:
-    // 36.4 -> 28.3; but 3 x 1370 without a mask: 26.5 -> 28.8), and in any case
-    // where a wave is long (4096 keys: 5477 rows, 5 heads, no mask 81.4 -> 63.2;
-    // 8 heads, 344 CTAs: 106.6 -> 97.9, while 430 lose). Lengths that only the
-    // device knows count as unlike: quarters of half a wave (2 x 1370 newest rows
-    // of 5480 and 2000, 6 heads: 45.7 -> 37.7; of 5480 twice: 47.8 -> 49.1).
+    // Split the keys while that many CTAs still run at once (two an SM) and each
+    // keeps 256 keys of an average sequence. Where a mask, or lengths that only
+    // the device knows, make up to two waves of tiles unlike, the long ones alone
+    // are split (ranked_tile): by two, or by four where that still runs at once
+    // and the streams are long. 7 images up to 1370 rows, 6 heads: 24.9 -> 23.0 us
+    // (all of them in halves 29.7); 1800, 1000 and 600 rows 31.9 -> 22.6; 5477
+    // rows causal, 6 heads 71.4 -> 47.3 (in halves 46.5); 3 x 1370 causal 23.2 ->
+    // 17.8, without a mask 26.2 -> 28.9, which the launch by clusters costs; 1370
+    // newest rows of 5480 and 2000 45.7 -> 39.0 (in quarters 37.2). A long wave
+    // of like tiles is split in halves (4096 keys: 5477 rows, 5 heads 81.4 ->
+    // 63.2; 8 heads, 344 CTAs, 106.6 -> 97.9; 430 would lose).
     const uint64_t keys = a.offsets != nullptr ? a.tokens / a.batch : a.tokens;
     const uint64_t ctas = units * p.heads;
     uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>({8, 2 * kSms / ctas, keys / 256}));
-    if (splits == 1 && ctas <= 370 &&
-        keys >= (p.mask != BL_MASK_NONE && ctas <= 2 * kSms ? 1536u : 4096u))
+    const bool unlike = p.mask != BL_MASK_NONE || (p.ragged && a.batch > 1);
+    if (a.key_splits == 0 && unlike && a.batch <= 32 && splits <= 2 && ctas <= 600 && keys >= 512) {
+        p.mixed = 1;
+        splits = splits == 2 && keys >= 1536 ? 4 : 2;
+    } else if (splits == 1 && ctas <= 370 && keys >= 4096) {
         splits = 2;
-    else if (splits == 2 && p.ragged && a.batch > 1 && keys >= 1536)
-        splits = 4;
+    }
     p.splits = static_cast<int>(a.key_splits ? a.key_splits : splits);
     if (units * p.heads * p.splits > 0x7FFFFFFFull)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: grid too large");

@@ -394,6 +394,20 @@ def test_every_tile_of_a_ragged_batch_is_found(batch, form, mask, last):
     Case(lens, heads=1, form=form, seed=batch).both(mask=mask, last_rows=last, **kw)
 
 
+@pytest.mark.parametrize("lens,heads,form", [
+    ([1500, 200, 64, 900], 2, "packed"), ([1500, 200, 0, 900], 2, "padded"),
+    ([1600, 300], 5, "padded"), ([1600, 1000], 5, "packed"), ([2000], 8, "packed")])
+@pytest.mark.parametrize("mask", [None, "causal", "prefix"])
+def test_long_tiles_are_split_beside_whole_ones(lens, heads, form, mask):
+    kw = {"prefix": [n // 3 for n in lens]} if mask == "prefix" else {}
+    c = Case(lens, heads=heads, kv=1, form=form, tokens=max(lens) if form == "padded" else None,
+             seed=41)
+    out = c.run(mask=mask, **kw)
+    c.check(out, mask=mask, **kw)
+    again = c.run(mask=mask, **kw)  # the same bits in every run
+    assert np.array_equal(out.float().cpu().numpy(), again.float().cpu().numpy())
+
+
 def test_padded_batch_without_lengths_and_strided_rows():
     import torch
     c = Case([96, 96, 96], heads=2, kv=1, form="padded", extra=3)
