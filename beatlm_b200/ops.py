@@ -314,6 +314,18 @@ def _row_stride(what, stride, rows):
     return stride if rows > 1 else 0
 
 
+def _out_code(what, out, out_dtype):
+    """The type code of the values a call stores in `out`: a floating tensor's
+    own, or for a container of bits (int16, int32) what `out_dtype` says, of the
+    container's size, since the kernel strides and stores by it."""
+    own = _T.code.get(out.dtype)
+    code = own if out_dtype is None else _TD[out_dtype]
+    if code is None or (own != code if out.dtype.is_floating_point
+                        else out.element_size() != (4 if code == N.BL_F32 else 2)):
+        raise ValueError("%s: %s results in an out of %s" % (what, out_dtype or "untyped", out.dtype))
+    return code
+
+
 def _launch(fn, args, tensor, stream):
     """Calls `fn` on `tensor`'s device, whichever device is current."""
     device = tensor.get_device()
@@ -450,9 +462,10 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
     ``[rows][heads + 2 kv_heads][64]``) packed rows. ``offsets`` (int32
     ``[batch + 1]``): packed sequences; otherwise ``batch`` (default: as many
     as ``lengths`` has, else 1) equal parts of the rows, ``lengths`` (int32
-    ``[batch]``) of each in use. ``out``: ``[rows][heads * 64]``. ``prefix``:
-    int32 ``[batch]``; ``slopes``: f32 ``[heads]``; ``positions``: f32
-    ``[rows][1 to 3 axes]``."""
+    ``[batch]``) of each in use. ``out``: ``[rows][heads * 64]``, a floating
+    tensor or a container of ``out_dtype``'s size. ``prefix``: int32
+    ``[batch]``; ``slopes``: f32 ``[heads]``; ``positions``: f32 ``[rows][1 to 3
+    axes]``."""
     _on_gpu("masked attention", qkv, out, offsets, lengths, prefix, slopes, positions)
     kv = heads if kv_heads is None else kv_heads
     shape, st = qkv.shape, qkv.stride()
@@ -500,7 +513,7 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
     return N.MaskedAttentionArgs(
         batch, tokens, heads, kv, 64, min(last_rows, 2 ** 31 - 1),
         0.125 if scale is None else scale, cap or 0.0, MASK[mask], _TD[qk_dtype], N.BL_F16,
-        _T.code[out.dtype] if out_dtype is None else _TD[out_dtype], qkv.data_ptr(),
+        _out_code("masked attention", out, out_dtype), qkv.data_ptr(),
         _row_stride("masked attention: qkv", st[0], rows), out.data_ptr(),
         _row_stride("masked attention: out", o_st[0], rows), None if offsets is None else offsets.data_ptr(),
         None if lengths is None else lengths.data_ptr(),
@@ -523,10 +536,6 @@ def masked_attention(qkv, *, heads, out=None, out_dtype=None, stream=None, **kw)
         s = torch.cuda.ExternalStream(stream, device=qkv.device) if isinstance(stream, int) else stream
         with torch.cuda.stream(s):  # (None: the current one)
             out = torch.zeros((qkv.shape[0], heads * 64), dtype=tdt, device=qkv.device)
-        out_dtype = None
-    elif out.dtype.is_floating_point:
-        if out_dtype is not None and _T.code.get(out.dtype) != _TD[out_dtype]:
-            raise ValueError("masked attention: out is %s, not %s" % (out.dtype, out_dtype))
         out_dtype = None
     a = masked_attention_args(qkv, heads=heads, out=out, out_dtype=out_dtype, **kw)
     if a.batch and a.tokens:

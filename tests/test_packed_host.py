@@ -124,3 +124,38 @@ def test_python_calls_refuse_cpu_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         ops.masked_attention(torch.zeros((2, 3, 64), dtype=torch.int16), heads=1,
                              out=torch.zeros((2, 64)))
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The calls' own checks, without a GPU: argument structs are made of CPU
+    tensors and nothing is launched."""
+    from beatlm_b200 import ops
+    monkeypatch.setattr(ops, "_on_gpu", lambda *a: None)
+    monkeypatch.setattr(ops, "_launch", lambda *a: pytest.fail("launched"))
+    return ops
+
+
+@pytest.mark.parametrize("container,out_dtype", [
+    ("int16", "f32"), ("float16", "f32"), ("bfloat16", "f32"), ("float16", "bf16"),
+    ("bfloat16", "f16"), ("float32", "f16"), ("int32", "bf16"), ("uint8", "f16"),
+    ("float64", "f32"), ("float64", None), ("int16", None), ("int32", None)])
+def test_an_output_of_another_type_or_size_is_refused(on_cpu, container, out_dtype):
+    """Four-byte results in two-byte rows would end behind the buffer."""
+    import torch
+    qkv = torch.zeros((5, 3, 64), dtype=torch.int16)
+    out = torch.zeros((5, 64), dtype=getattr(torch, container))
+    for call in (on_cpu.masked_attention_args, on_cpu.masked_attention):
+        with pytest.raises(ValueError, match="masked attention: .* results in an out of"):
+            call(qkv, heads=1, out=out, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("container,out_dtype,code", [
+    ("float32", None, N.BL_F32), ("float16", None, N.BL_F16), ("bfloat16", "bf16", N.BL_BF16),
+    ("int16", "f16", N.BL_F16), ("int16", "bf16", N.BL_BF16), ("int32", "f32", N.BL_F32)])
+def test_outputs_and_containers_that_fit(on_cpu, container, out_dtype, code):
+    import torch
+    a = on_cpu.masked_attention_args(torch.zeros((5, 3, 64), dtype=torch.int16), heads=1,
+                                     out=torch.zeros((5, 64), dtype=getattr(torch, container)),
+                                     out_dtype=out_dtype)
+    assert a.out_dtype == code
