@@ -1261,9 +1261,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             const float sum = ok ? ex2(m_used - ref) * l + ex2(other - ref) * tail->odd_sum[row] : 0.0f;
             if (splits > 1) {
                 // the ring is free here: the last PV is complete, so every copy
-                // has landed and been read
+                // has landed and been read, and every zero behind the sequence's
+                // end is written, which the arrivals release to the CTAs that
+                // store over them
                 __syncwarp();
-                cluster_arrive();
+                cluster_arrive_release();
                 cluster_wait();
                 // the row's O, maximum and sum into its owner's ring; its vectors
                 // rotated, so that a warp's stores spread over the banks
@@ -1311,7 +1313,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         // (the same bits in every run) and no CTA reads another's memory.
         __syncwarp();
         if (warp < kSoftmaxWarp0 || warp >= kSoftmaxWarp0 + 4) {
-            cluster_arrive();
+            cluster_arrive_release();
             cluster_wait();
         }
         __syncwarp();

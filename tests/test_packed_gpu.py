@@ -408,6 +408,21 @@ def test_long_tiles_are_split_beside_whole_ones(lens, heads, form, mask):
     assert np.array_equal(out.float().cpu().numpy(), again.float().cpu().numpy())
 
 
+@pytest.mark.parametrize("splits", [2, 4, 7])
+def test_split_parts_land_in_rings_that_are_free(splits):
+    """Key tiles that end with their sequence have rows of V zeroed in the ring
+    that other CTAs then store parts into: many launches, one after the other,
+    give the same bits, and the right ones."""
+    import torch
+    c = Case([449, 130, 65, 321, 700], heads=3, seed=43)
+    outs = [torch.full((c.rows, 192), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(40)]
+    for o in outs:
+        c.run(out=o, key_splits=splits)
+    for o in outs:
+        assert torch.equal(o, outs[0])
+    c.check(outs[0])
+
+
 def test_padded_batch_without_lengths_and_strided_rows():
     import torch
     c = Case([96, 96, 96], heads=2, kv=1, form="padded", extra=3)
