@@ -888,13 +888,17 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     auto first_key = [&](int i) { return (t0 + (i <= pivot ? pivot - i : i)) * BN; };
 
     // One lane waits and the vote hands its outcome to the warp, unless the
-    // barrier is past that phase already.
+    // barrier is past that phase already. A vote orders no memory: __syncwarp
+    // does, so that what came before the barrier's arrivals (R, sums in shared
+    // memory) is there for the lanes that did not wait themselves.
     const bool elected = elect_one();
     auto wait_warp = [&](uint64_t* bar, int parity, uint32_t code, uint32_t where) -> bool {
         if (__all_sync(kFull, mbar_try_wait(smem_u32(bar), parity))) return true;
         bool r = true;
         if (elected) r = mbar_wait(smem_u32(bar), parity, abort, p.status, code, where);
-        return __all_sync(kFull, r);
+        r = __all_sync(kFull, r);
+        __syncwarp();
+        return r;
     };
     if (warp == 0) {
         // ------------------------------------------------------ producer

@@ -458,6 +458,26 @@ def test_a_dominant_score_late_in_the_sequence():
     c.both(mask="causal")
 
 
+@pytest.mark.parametrize("slope", [None, -0.25])
+def test_the_maximum_changes_hands_with_every_tile(slope):
+    """Scores that rise from key tile to key tile (or, with a negative slope, away
+    from the row): each of the two streams of a row's softmax takes a new
+    reference from the other every time, the same bits in many launches."""
+    import torch
+    c = Case([1000, 260], heads=2, qk="f16", seed=47)
+    kw = {"slopes": np.full(2, slope, np.float32)} if slope else {}
+    if not slope:
+        x = c.qkv.view(torch.float16)
+        x[:, 2:4, 0] = (torch.arange(c.rows, device="cuda") / 20.0).half()[:, None]
+        x[:, :2, 0] = 8.0  # a score grows by 3.2 a tile of 64 keys
+        x = x.double().cpu().numpy()
+        c.q, c.k = x[:, :2], x[:, 2:4]
+    outs = [c.run(**kw) for _ in range(20)]
+    for o in outs:
+        assert torch.equal(o, outs[0])
+    c.check(outs[0], **kw)
+
+
 def test_offsets_and_lengths_that_point_outside_are_clamped():
     import torch
     c = Case([50, 60], heads=1, gap=0, seed=1)
