@@ -1405,6 +1405,20 @@ int validate(const bl_masked_attention_args& a) {
     if (orow < ow || (orow * dtype_size(a.out_dtype)) % 16 != 0 || orow >= (1ull << 40) ||
         (reinterpret_cast<uintptr_t>(a.out) & 15u))
         return fail(BL_ERR_INVALID, "masked attention: output stride or alignment");
+    // Rows of K and V are read until the last CTA is done, so the output lies
+    // apart from qkv's rows: in memory of its own or in columns of one wider row.
+    // Q alone may be written over, by its own results in its own places: a CTA
+    // (or the cluster that shares its keys) stores a row's after the last use of
+    // its Q, which nobody else reads.
+    const uintptr_t px = reinterpret_cast<uintptr_t>(a.qkv), po = reinterpret_cast<uintptr_t>(a.out);
+    const uint64_t esz = dtype_size(a.out_dtype), xs = row * 2, os = orow * esz;
+    if (px < po + (rows - 1) * os + ow * esz && po < px + (rows - 1) * xs + width * 2) {
+        const uint64_t d = (px < po ? po - px : xs - (px - po) % xs) % xs;
+        const bool over_q = px == po && esz == 2 && (xs == os || rows == 1);
+        const bool columns = xs == os && d >= width * 2 && d + ow * esz <= xs;
+        if (!over_q && !columns)
+            return fail(BL_ERR_INVALID, "masked attention: out overlaps qkv");
+    }
     for (const void* q : {static_cast<const void*>(a.offsets), static_cast<const void*>(a.lengths),
                           static_cast<const void*>(a.prefix), static_cast<const void*>(a.slopes),
                           static_cast<const void*>(a.positions)})

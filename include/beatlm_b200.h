@@ -607,8 +607,10 @@ int bl_rope(const bl_rope_args* args, void* stream);
  * value); the probabilities are rounded to f16 for the tensor cores (as in
  * bl_attention). key_splits: how many CTAs share a tile's keys (a cluster,
  * combined on chip): 0 = automatic, at most 8. head_dim must be 64; qkv and out
- * 16-byte aligned with strides of 16-byte multiples. Enqueues on `stream`;
- * allocates nothing; no workspace, and the same bits in every run.
+ * 16-byte aligned with strides of 16-byte multiples. out lies apart from qkv
+ * (columns of one wider row count), or 16-bit results replace Q: out = qkv with
+ * its stride. Enqueues on `stream`; allocates nothing; no workspace, and the
+ * same bits in every run.
  */
 enum { BL_MASK_NONE = 0, BL_MASK_CAUSAL = 1, BL_MASK_PREFIX = 2 };
 typedef struct bl_masked_attention_args {

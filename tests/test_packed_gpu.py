@@ -432,6 +432,21 @@ def test_padded_batch_without_lengths_and_strided_rows():
     assert torch.all(out[:, 128:] == 7.0)
 
 
+@pytest.mark.parametrize("last,splits", [(0, 0), (0, 3), (0, 1), (2, 0), (2, 2), (100, 0)])
+def test_results_in_the_places_of_q(last, splits):
+    """And in columns beside the rows they come from."""
+    import torch
+    c = Case([300, 77, 5, 130], heads=4, kv=2, seed=51, extra=4)
+    kw = dict(mask="causal", last_rows=last, key_splits=splits)
+    want = c.run(**kw)
+    flat = c.buf.view(torch.bfloat16).reshape(c.rows, -1)  # 8 heads of Q|K|V, 4 more
+    beside = c.run(out=flat[:, 512:768], **kw)
+    over = c.run(out=flat[:, :256], **kw)
+    done = (want != 7.0).any(1)
+    assert torch.equal(beside[done], want[done]) and torch.equal(over[done], want[done])
+    assert int(done.sum()) == sum(min(last or n, n) for n in (300, 77, 5, 130))
+
+
 def test_a_sequence_that_overflows_keeps_to_itself():
     """Infinite scores make their own rows NaN, as the formula does, and no others."""
     import torch

@@ -159,3 +159,29 @@ def test_outputs_and_containers_that_fit(on_cpu, container, out_dtype, code):
                                      out=torch.zeros((5, 64), dtype=getattr(torch, container)),
                                      out_dtype=out_dtype)
     assert a.out_dtype == code
+
+
+# 128 rows of 512 values of Q|K|V (1024 bytes), 256 values of output (512 bytes in 16 bits)
+@pytest.mark.parametrize("kw", [
+    dict(out=A + 512, out_row_stride=512), dict(out=A + 768, out_row_stride=512), dict(out=A),
+    dict(out=A, out_row_stride=512, out_dtype=N.BL_F32), dict(out=A + 127 * 1024 + 1008),
+    dict(out=A - 127 * 512), dict(out=A, qkv_row_stride=768, out_row_stride=512),
+    dict(out=A + 1008, qkv_row_stride=768, out_row_stride=768),
+    dict(out=A + 1040, qkv_row_stride=768, out_row_stride=768),
+    dict(out=A - 496, qkv_row_stride=768, out_row_stride=768),
+    dict(out=A + 1024, qkv_row_stride=768, out_row_stride=384, out_dtype=N.BL_F32),
+    dict(out=A + 16, batch=1, tokens=1), dict(out=A, batch=1, tokens=1, out_dtype=N.BL_F32)])
+def test_an_output_over_rows_still_read_is_refused(kw):
+    with pytest.raises(N.BackendError, match="out overlaps qkv"):
+        _call(N.lib().bl_masked_attention, _attn(**kw))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=A, out_row_stride=512), dict(out=A, batch=1, tokens=1),
+    dict(out=A + 128 * 1024), dict(out=A - 128 * 512),
+    dict(out=A + 1024, qkv_row_stride=768, out_row_stride=768),
+    dict(out=A - 512, qkv_row_stride=768, out_row_stride=768)])
+def test_outputs_apart_and_over_q_pass_the_overlap_check(kw):
+    """(No GPU here: what comes after the check of arguments fails, otherwise.)"""
+    with pytest.raises(N.BackendError, match="4-byte"):
+        _call(N.lib().bl_masked_attention, _attn(lengths=4 * A + 2, **kw))
