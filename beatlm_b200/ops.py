@@ -280,7 +280,7 @@ class _Torch:
     def __getattr__(self, name):  # the first use of any of them
         import torch
         self.code = {torch.float32: N.BL_F32, torch.float16: N.BL_F16, torch.bfloat16: N.BL_BF16}
-        self.int32, self.float32 = torch.int32, torch.float32
+        self.int32, self.float32, self.float16 = torch.int32, torch.float32, torch.float16
         self.current_device = torch.cuda.current_device
         self.raw_stream = torch._C._cuda_getCurrentRawStream
         return self.__dict__[name]
@@ -459,7 +459,8 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
                           mask=None, prefix=None, cap=None, slopes=None, positions=None,
                           key_splits=0):
     """``qkv``: 16-bit ``[rows][(heads + 2 kv_heads) * 64]`` (or
-    ``[rows][heads + 2 kv_heads][64]``) packed rows. ``offsets`` (int32
+    ``[rows][heads + 2 kv_heads][64]``) packed rows, a float16 tensor or an
+    int16 container (V is f16 beside Q and K of ``qk_dtype``). ``offsets`` (int32
     ``[batch + 1]``): packed sequences; otherwise ``batch`` (default: as many
     as ``lengths`` has, else 1) equal parts of the rows, ``lengths`` (int32
     ``[batch]``) of each in use. ``out``: ``[rows][heads * 64]``, a floating
@@ -478,6 +479,9 @@ def masked_attention_args(qkv, *, heads, out, kv_heads=None, batch=None, offsets
             width < (heads + 2 * kv) * 64:
         raise ValueError("masked attention: qkv is %s (strides %s) of %s for %d heads and %d K/V "
                          "heads of 64 side by side" % (tuple(shape), st, qkv.dtype, heads, kv))
+    if qkv.dtype.is_floating_point and not (qkv.dtype is _T.float16 and qk_dtype == "f16"):
+        raise ValueError("masked attention: %s Q and K beside f16 V in a tensor of %s"
+                         % (qk_dtype, qkv.dtype))
     rows = shape[0]
     o_shape, o_st = out.shape, out.stride()
     if len(o_shape) != 2 or o_shape[0] < rows or o_shape[1] < heads * 64 or o_st[1] != 1:

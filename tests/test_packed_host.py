@@ -185,3 +185,18 @@ def test_outputs_apart_and_over_q_pass_the_overlap_check(kw):
     """(No GPU here: what comes after the check of arguments fails, otherwise.)"""
     with pytest.raises(N.BackendError, match="4-byte"):
         _call(N.lib().bl_masked_attention, _attn(lengths=4 * A + 2, **kw))
+
+
+@pytest.mark.parametrize("tensor,qk_dtype", [
+    ("bfloat16", "f16"), ("bfloat16", "bf16"), ("float16", "bf16")])
+def test_rows_of_another_type_than_they_are_read_as_are_refused(on_cpu, tensor, qk_dtype):
+    """A bfloat16 tensor's V is not f16, whatever its Q and K are read as."""
+    import torch
+    out = torch.zeros((5, 64), dtype=torch.float16)
+    for shape in ((5, 3, 64), (5, 192)):
+        qkv = torch.zeros(shape, dtype=getattr(torch, tensor))
+        for call in (on_cpu.masked_attention_args, on_cpu.masked_attention):
+            with pytest.raises(ValueError, match="beside f16 V in a tensor of torch." + tensor):
+                call(qkv, heads=1, out=out, qk_dtype=qk_dtype)
+    for t, qk in ((torch.float16, "f16"), (torch.int16, "f16"), (torch.int16, "bf16")):
+        on_cpu.masked_attention_args(torch.zeros((5, 192), dtype=t), heads=1, out=out, qk_dtype=qk)
