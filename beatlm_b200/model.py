@@ -869,6 +869,7 @@ class PackedEncoder:
         zeros = lambda shape, dt: torch.zeros(shape, dtype=dt, device=device)
         self.grids = zeros((images, 3), torch.int32)
         self.offsets = zeros((images + 1,), torch.int32)
+        self._given = zeros((images + 1,), torch.int32)  # offsets among the rows of a call
         self.image_of = zeros((capacity,), torch.int32)
         self.positions = zeros((capacity, 3), torch.float32)
         self.patches = zeros((capacity, cfg.k_pad), td)
@@ -925,7 +926,9 @@ class PackedEncoder:
         ``grids``: int32 ``[n][3]`` (t, h, w), n at most ``images``. Returns
         the normalised rows (device f32 ``[capacity][dim]``; image i's are
         ``offsets[i]`` to ``offsets[i + 1]``, those behind the last hold
-        nothing of use). Nothing waits for the host."""
+        nothing of use). Nothing waits for the host, so grids that ask for more
+        rows than are given read zeros there, and the device status word
+        records it (0x50, as for rows past the capacity)."""
         n, rows = grids.shape[0], patches.shape[0]
         if n > self.images or rows > self.capacity or patches.shape[1] != self.cfg.k_pad:
             raise ValueError("%d images with %s patch rows in an encoder for %d and [%d][%d]"
@@ -935,6 +938,9 @@ class PackedEncoder:
             self.grids[:n].copy_(grids)
             self.grids[n:].zero_()
             self.patches[:rows].copy_(patches)
+            if rows < self.capacity:  # what is left of another call's rows
+                self.patches[rows:].zero_()
+                ops.pack(self.grids, offsets=self._given, capacity=max(rows, 1))
             self.program().encode_all(None)
         return self.out
 

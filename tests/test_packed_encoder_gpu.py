@@ -146,3 +146,30 @@ def test_without_masks_it_is_the_dense_attention(t, h):
     got = ops.masked_attention(qkv.reshape(t, 3 * h, 64), heads=h, qk_dtype="bf16",
                                out_dtype="f32").double()
     assert float((got - want).norm() / want.norm()) <= 2e-3
+
+
+def test_rows_that_were_not_given_are_zeros_and_recorded():
+    """Grids that ask for more patch rows than a call gives: what is missing is
+    zeros, never the rows of the batch before, and the status word says so."""
+    import torch
+    import beatlm_b200 as bl
+    from beatlm_b200 import model as M
+    cfg = _cfg()
+    w = _weights(cfg, 6)
+    enc = M.PackedEncoder(cfg, w, capacity=260, images=3, dtype="f16")
+    dev = lambda x: torch.from_numpy(x).half().cuda()  # noqa: E731
+    sizes = lambda g: torch.tensor(g, dtype=torch.int32, device="cuda")  # noqa: E731
+    enc.forward(dev(_patches(cfg, 250, 12)), sizes([(1, 10, 25)]))
+    torch.cuda.synchronize()
+    assert bl.status(reset=True).code == 0
+    grids, given = [(1, 8, 9), (1, 11, 12)], 100
+    x = _patches(cfg, 72 + 132, 13)
+    x[given:] = 0.0
+    got = enc.forward(dev(x[:given]), sizes(grids))[:204].double().cpu().numpy()
+    assert bl.status(reset=True).code == 0x50
+    want, _ = _reference(cfg, w, x[:, :cfg.taps], grids, (16, 16))
+    rel = np.linalg.norm(got - want) / np.linalg.norm(want)
+    assert rel <= cfg.layers * ROUNDINGS * STEP, rel
+    enc.forward(dev(x[:204]), sizes(grids))
+    torch.cuda.synchronize()
+    assert bl.status(reset=True).code == 0
