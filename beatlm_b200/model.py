@@ -847,12 +847,14 @@ class PackedEncoder:
         """``weights`` as ``Encoder`` takes them (class token and learned
         positions are not used). ``sections``: rotary pairs of the (time,
         height, width) axes, default half of the head's pairs for height and
-        half for width; two numbers are (height, width). ``mask``, ``cap`` and
-        ``slopes`` (one a head, a bias by distance on the patch grid): as
-        ``ops.masked_attention``."""
+        half for width; two numbers are (height, width). ``mask`` (None or
+        "causal"), ``cap`` and ``slopes`` (one a head, a bias by distance on
+        the patch grid): as ``ops.masked_attention``."""
         import torch
         if cfg.head_dim != 64:
             raise ValueError("heads of 64, not %d" % cfg.head_dim)
+        if mask not in (None, "none", "causal"):
+            raise ValueError("mask %r: the encoder attends to whole images or causally" % (mask,))
         td = torch.bfloat16 if dtype == "bf16" else torch.float16
         pairs = cfg.head_dim // 2
         sections = tuple(sections or (pairs // 2, pairs - pairs // 2))

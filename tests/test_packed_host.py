@@ -2,6 +2,7 @@
 away on the host, before anything is launched (no GPU needed)."""
 import ctypes
 
+import numpy as np
 import pytest
 
 from beatlm_b200 import _native as N
@@ -200,3 +201,21 @@ def test_rows_of_another_type_than_they_are_read_as_are_refused(on_cpu, tensor, 
                 call(qkv, heads=1, out=out, qk_dtype=qk_dtype)
     for t, qk in ((torch.float16, "f16"), (torch.int16, "f16"), (torch.int16, "bf16")):
         on_cpu.masked_attention_args(torch.zeros((5, 192), dtype=t), heads=1, out=out, qk_dtype=qk)
+
+
+def _encoder(**kw):
+    from beatlm_b200 import model as M
+    cfg = M.ViTConfig(dim=128, heads=2, mlp=256, layers=0, patch=4, side=8, cin=3, out_indices=())
+    n = lambda *s: np.zeros(s, np.float32)  # noqa: E731
+    w = {"blocks": [], "patch_w": n(cfg.taps, 128), "patch_b": n(128), "norm_g": n(128),
+         "norm_b": n(128)}
+    return cfg, M.PackedEncoder(cfg, w, capacity=50, images=4, dtype="f16", device="cpu", **kw)
+
+
+@pytest.mark.parametrize("mask", ["prefix", "document", 1])
+def test_the_packed_encoder_refuses_masks_it_has_no_way_to_run(mask):
+    """A prefix mask needs lengths, which the encoder does not take."""
+    with pytest.raises(ValueError, match="mask"):
+        _encoder(mask=mask)
+    for m in (None, "none", "causal"):
+        _encoder(mask=m)
