@@ -932,10 +932,12 @@ class PackedEncoder:
         rows than are given read zeros there, and the device status word
         records it (0x50, as for rows past the capacity)."""
         n, rows = grids.shape[0], patches.shape[0]
-        if n > self.images or rows > self.capacity or patches.shape[1] != self.cfg.k_pad:
-            raise ValueError("%d images with %s patch rows in an encoder for %d and [%d][%d]"
-                             % (n, tuple(patches.shape), self.images, self.capacity,
-                                self.cfg.k_pad))
+        if n > self.images or rows > self.capacity or tuple(patches.shape[1:]) != (self.cfg.k_pad,) \
+                or tuple(grids.shape[1:]) != (3,) or not patches.is_floating_point():
+            raise ValueError("%d images with %s patch rows of %s (sizes %s) in an encoder for %d "
+                             "and [%d][%d]" % (n, tuple(patches.shape), patches.dtype,
+                                               tuple(grids.shape), self.images, self.capacity,
+                                               self.cfg.k_pad))
         with _on_stream(stream):
             self.grids[:n].copy_(grids)
             self.grids[n:].zero_()

@@ -219,3 +219,16 @@ def test_the_packed_encoder_refuses_masks_it_has_no_way_to_run(mask):
         _encoder(mask=mask)
     for m in (None, "none", "causal"):
         _encoder(mask=m)
+
+
+def test_the_packed_encoder_refuses_sizes_and_patches_of_other_forms():
+    """Sizes of one column would be spread over (t, h, w), bits in an integer
+    container taken for numbers."""
+    import torch
+    cfg, enc = _encoder()
+    rows, sizes = torch.zeros((6, cfg.k_pad), dtype=torch.float16), torch.ones((2, 3), dtype=torch.int32)
+    for r, g in ((rows, sizes[:, :1]), (rows, sizes[0]), (rows, torch.ones((2, 2, 3))),
+                 (rows.view(torch.int16), sizes), (rows[None], sizes), (rows[:, :5], sizes),
+                 (rows[0], sizes)):
+        with pytest.raises(ValueError, match="images with"):
+            enc.forward(r, g)
