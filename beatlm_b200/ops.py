@@ -67,6 +67,8 @@ def attention_args(qkv, *, tokens, heads, out, head_dim=64, batch=1, qk_dtype="f
     r0, r1 = rows or (0, tokens)
     h0, h1 = head_range or (0, heads)
     odt = _TD[out_dtype] if out_dtype is not None else _dt(out)
+    if out.element_size() != (4 if odt == N.BL_F32 else 2):  # it is stored by the type's size
+        raise ValueError("attention: %s results in an out of %s" % (out_dtype, out.dtype))
     return N.AttentionArgs(batch=batch, tokens=tokens, heads=heads, head_dim=head_dim,
                            head_begin=h0, head_end=h1, row_begin=r0, row_end=r1, scale=scale,
                            qk_dtype=_TD[qk_dtype], v_dtype=N.BL_F16, out_dtype=odt,

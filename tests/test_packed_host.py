@@ -232,3 +232,17 @@ def test_the_packed_encoder_refuses_sizes_and_patches_of_other_forms():
                  (rows[0], sizes)):
         with pytest.raises(ValueError, match="images with"):
             enc.forward(r, g)
+
+
+@pytest.mark.parametrize("container,out_dtype", [
+    ("int16", "f32"), ("float16", "f32"), ("uint8", "f16"), ("float32", "bf16")])
+def test_the_dense_attention_refuses_outputs_of_another_size(container, out_dtype):
+    import torch
+    from beatlm_b200 import ops
+    qkv = torch.zeros((1, 5, 3, 1, 64), dtype=torch.int16)
+    out = torch.zeros((1, 5, 64), dtype=getattr(torch, container))
+    with pytest.raises(ValueError, match="attention: .* results in an out of"):
+        ops.attention_args(qkv, tokens=5, heads=1, out=out, out_dtype=out_dtype)
+    for fits, name in ((torch.int16, "bf16"), (torch.float16, None), (torch.float32, "f32")):
+        ops.attention_args(qkv, tokens=5, heads=1, out=torch.zeros((1, 5, 64), dtype=fits),
+                           out_dtype=name)
