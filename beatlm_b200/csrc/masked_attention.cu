@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "host.h"
@@ -1381,6 +1382,12 @@ int validate(const bl_masked_attention_args& a) {
         return fail(BL_ERR_INVALID, "masked attention: cap must be finite, 0 for none");
     if (a.cap > 0.0f && static_cast<double>(a.scale) > 1e6 * a.cap)  // the series' coefficients
         return fail(BL_ERR_UNSUPPORTED, "masked attention: cap below a millionth of the scale");
+    // the constants that params_of makes of them
+    const double unit = a.cap > 0.0f ? static_cast<double>(a.scale) / a.cap : 0.0;
+    if (std::max({a.scale * 1.5, a.cap * 1.5, a.scale * std::pow(unit, 6) * 0.08}) >
+        std::numeric_limits<float>::max())
+        return fail(BL_ERR_UNSUPPORTED, "masked attention: scale %g, cap %g: constants leave 32 bits",
+                    a.scale, a.cap);
     if (a.mask < BL_MASK_NONE || a.mask > BL_MASK_PREFIX)
         return fail(BL_ERR_INVALID, "masked attention: mask %d", a.mask);
     if ((a.mask == BL_MASK_PREFIX) != (a.prefix != nullptr))

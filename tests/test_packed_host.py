@@ -246,3 +246,14 @@ def test_the_dense_attention_refuses_outputs_of_another_size(container, out_dtyp
     for fits, name in ((torch.int16, "bf16"), (torch.float16, None), (torch.float32, "f32")):
         ops.attention_args(qkv, tokens=5, heads=1, out=torch.zeros((1, 5, 64), dtype=fits),
                            out_dtype=name)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(scale=1e4, cap=0.0101),  # scale (scale / cap)^6, the last coefficient of the series
+    dict(scale=1.0, cap=3e38), dict(scale=3e38), dict(scale=3e38, cap=1e36)])
+def test_scores_whose_constants_leave_32_bits_are_refused(kw):
+    """An infinite constant times a score of zero is NaN."""
+    with pytest.raises(N.BackendError, match="32 bits"):
+        _call(N.lib().bl_masked_attention, _attn(**kw))
+    with pytest.raises(N.BackendError, match="4-byte"):  # well within them
+        _call(N.lib().bl_masked_attention, _attn(scale=1e3, cap=0.00101, lengths=4 * A + 2))
