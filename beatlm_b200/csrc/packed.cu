@@ -345,8 +345,8 @@ __device__ __forceinline__ void turn_pairs(Vec<T, kVec>& a, Vec<T, kVec>& b, con
 // What bounds it is memory: each value read once and written once. The angles
 // are few beside the values (one a row and pair, against one pair a head), but
 // dear: formed in 64 bits in half turns and reduced to [-1, 1] before the
-// 32-bit sincospif, so that positions of 10^6 and more lose nothing the result
-// could hold. A tile's cosines and sines are made once, into one of two shared
+// 32-bit sincospif, whose results are corrected for the rounding of its argument,
+// so that positions of 10^6 and more lose nothing the result could hold. A tile's cosines and sines are made once, into one of two shared
 // tables (so one barrier a tile is enough), while the tile's values are on
 // their way; a thread keeps the frequency of its pair over all its tiles.
 // 60280 rows x 32 heads x 64 in bf16 (494 MB): 75.9 us, the rate of a copy.
@@ -405,10 +405,15 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeP
             if (r0 + k >= p.rows) break;
             double h = static_cast<double>(p.pos[(r0 + k) * p.pos_stride + axis]) * turn;
             h -= 2.0 * rint(0.5 * h);
+            // the 32-bit angle's functions, turned on by what it left out (below
+            // 10^-7 radians, so to first order)
+            const float near = static_cast<float>(h);
+            const float rest = static_cast<float>((h - near) * 3.14159265358979323846);
             float sn, cn;
-            sincospif(static_cast<float>(h), &sn, &cn);
-            cs[2 * k * p.pairs + pair] = cn;
-            cs[(2 * k + 1) * p.pairs + pair] = p.inverse ? -sn : sn;
+            sincospif(near, &sn, &cn);
+            const float sine = fmaf(cn, rest, sn);
+            cs[2 * k * p.pairs + pair] = fmaf(-sn, rest, cn);
+            cs[(2 * k + 1) * p.pairs + pair] = p.inverse ? -sine : sine;
         }
         __syncthreads();
         if (mine) {

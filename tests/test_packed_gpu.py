@@ -211,6 +211,29 @@ def test_the_inverse_rotation_is_the_gradient(pairing):
         assert abs(float(diff) - float(grad[at])) <= 128 * 8 * 2.0 ** -23
 
 
+@pytest.mark.parametrize("pairing", ["half", "adjacent", "axis_half"])
+def test_cosines_and_sines_are_good_to_their_own_size(pairing):
+    """Pairs (1, 0) turn to (cos, sin) themselves: each within 2 ulp (the function),
+    half a one (its correction for what the angle's 32 bits left out) and the 64-bit
+    angle's own error, small sines of angles near a half turn too."""
+    import torch
+    from beatlm_b200 import ops
+    rows, sections = 1500, (16, 16)
+    g = torch.Generator(device="cuda").manual_seed(77)
+    pos = torch.rand((rows, 2), generator=g, device="cuda") * 2000 - 1000
+    x = torch.zeros((rows, 1, 64), device="cuda")
+    lows = [lo for _, _, lo, _ in ref.pairs(64, sections, pairing)]
+    x[:, :, lows] = 1.0
+    got = ops.rope(x, pos, sections=sections, theta=100.0, pairing=pairing, out=torch.empty_like(x))
+    want, _ = ref.rope(x.double().cpu().numpy(), pos.double().cpu().numpy(), sections, 100.0,
+                       pairing, False)
+    size = np.maximum(np.abs(want), 2.0 ** -100)
+    ulp = 2.0 ** (np.floor(np.log2(size)) - 23)
+    bound = 2.5 * ulp * (1 + 2.0 ** -20) + 1000 * 2.0 ** -50 + 2.0 ** -43
+    off = np.abs(got.double().cpu().numpy() - want)
+    assert np.all(off <= bound), (off / bound).max()
+
+
 # ------------------------------------------------------------------ attention
 
 class Case:
