@@ -404,6 +404,54 @@ def test_key_splits(splits, last):
     assert np.array_equal(c.run(**kw).float().cpu().numpy(), c.run(**kw).float().cpu().numpy())
 
 
+def _places(c, axes, seed):
+    """Places of a case's rows on a grid, some of them off it; NaN behind its sequences."""
+    rng = np.random.default_rng(seed)
+    pos = rng.integers(0, 40, (c.rows, axes)).astype(np.float64)
+    pos[::3] += rng.random((c.rows, axes))[::3]
+    dead = np.ones(c.rows, bool)
+    for b, e in c.where:
+        dead[b:e] = False
+    pos[dead] = np.nan
+    return pos.astype(np.float32).astype(np.float64)
+
+
+@pytest.mark.parametrize("axes", [1, 2, 3])
+@pytest.mark.parametrize("mask", [None, "causal", "prefix"])
+@pytest.mark.parametrize("cap", [None, 20.0])
+@pytest.mark.parametrize("last", [0, 1, 4, 40])
+def test_places_under_masks_and_of_newest_rows(axes, mask, cap, last):
+    """Few rows (up to 16 a K/V head) and tiles; prefixes that end inside one."""
+    lens = [300, 0, 67, 1, 129]
+    c = Case(lens, heads=4, kv=2, seed=axes, form="padded" if axes == 2 else "packed")
+    kw = {"prefix": [100, 3, 70, 0, 65]} if mask == "prefix" else {}
+    c.both(slopes=np.array(SLOPES[:4], np.float32), positions=_places(c, axes, axes), cap=cap,
+           mask=mask, last_rows=last, **kw)
+
+
+@pytest.mark.parametrize("splits", [2, 3, 8])
+@pytest.mark.parametrize("last", [0, 1, 100])
+@pytest.mark.parametrize("cap,axes", [(20.0, None), (20.0, 0), (None, 2), (2.0, 3)])
+def test_key_splits_with_caps_and_places(splits, last, cap, axes):
+    c = Case([700, 20, 129], heads=2, seed=4)
+    kw = dict(mask="causal", last_rows=last, key_splits=splits, cap=cap)
+    if axes is not None:
+        kw["slopes"] = np.array(SLOPES[3:5], np.float32)
+    if axes:
+        kw["positions"] = _places(c, axes, 9)
+    c.both(**kw)
+
+
+@pytest.mark.parametrize("form", ["packed", "padded"])
+@pytest.mark.parametrize("last", [1, 20])
+def test_newest_rows_of_many_sequences(form, last):
+    rng = np.random.default_rng(last)
+    for batch in (32, 33, 70):
+        lens = [int(v) for v in rng.integers(0, 500, batch)]
+        c = Case(lens, heads=2, kv=1, form=form, tokens=512, seed=batch)
+        c.both(mask="causal", last_rows=last, slopes=np.array(SLOPES[:2], np.float32))
+
+
 @pytest.mark.parametrize("batch", [2, 31, 32, 33])
 @pytest.mark.parametrize("form", ["packed", "padded"])
 @pytest.mark.parametrize("mask", [None, "causal", "prefix"])
@@ -429,6 +477,19 @@ def test_long_tiles_are_split_beside_whole_ones(lens, heads, form, mask):
     c.check(out, mask=mask, **kw)
     again = c.run(mask=mask, **kw)  # the same bits in every run
     assert np.array_equal(out.float().cpu().numpy(), again.float().cpu().numpy())
+
+
+@pytest.mark.parametrize("lens,heads,form", [
+    ([1500, 200, 64, 900], 2, "packed"), ([1600, 300], 5, "padded"), ([2000], 8, "packed")])
+@pytest.mark.parametrize("mask", [None, "causal", "prefix"])
+@pytest.mark.parametrize("axes,cap", [(0, None), (0, 20.0), (2, None), (3, 20.0)])
+def test_long_tiles_are_split_with_a_bias(lens, heads, form, mask, axes, cap):
+    """The nearest keys come first within each part."""
+    kw = {"prefix": [n // 3 for n in lens]} if mask == "prefix" else {}
+    c = Case(lens, heads=heads, kv=1, form=form, seed=45)
+    if axes:
+        kw["positions"] = _places(c, axes, 3)
+    c.both(mask=mask, cap=cap, slopes=np.array(SLOPES[:heads], np.float32), **kw)
 
 
 @pytest.mark.parametrize("splits", [2, 4, 7])
