@@ -173,3 +173,75 @@ def test_rows_that_were_not_given_are_zeros_and_recorded():
     enc.forward(dev(x[:204]), sizes(grids))
     torch.cuda.synchronize()
     assert bl.status(reset=True).code == 0
+
+
+def _formulas(cfg, weights, patches, grids, dtype="f16", sections=(16, 16), pairing="axis_half",
+              normalized=False, **attn):
+    """_reference for every option, operands rounded as `dtype` holds them."""
+    from scipy.special import erf
+    from beatlm_b200.model import _round
+    held = lambda a: np.asarray(_round(np.asarray(a, np.float32), dtype), np.float64)  # noqa: E731
+    off, _, pos = ref.pack(grids, patches.shape[0], 0, normalized)
+    where = ref.spans(len(grids), patches.shape[0], offsets=off)
+    x = held(patches) @ held(weights["patch_w"]) + weights["patch_b"]
+    if attn.get("slopes") is not None:
+        attn["positions"] = pos
+    d, m, h = cfg.dim, cfg.mlp, cfg.heads
+    turn = lambda t: ref.rope(t, pos[:, 3 - len(sections):], sections, 100.0, pairing, False)[0]  # noqa: E731
+    for w in weights["blocks"]:
+        mat = lambda k, a, b: held(w[k]).reshape(a, b)  # noqa: E731
+        qkv = _ln(x, w["norm1_g"], w["norm1_b"], cfg.eps) @ mat("qkv_w", d, 3 * d) + w["qkv_b"]
+        q, k, v = (qkv[:, i * d:(i + 1) * d].reshape(-1, h, 64) for i in range(3))
+        o, _, _ = ref.attention(turn(q), turn(k), v, where, **attn)
+        x = x + w["ls1"] * (o.reshape(-1, d) @ mat("proj_w", d, d) + w["proj_b"])
+        hid = _ln(x, w["norm2_g"], w["norm2_b"], cfg.eps) @ mat("fc1_w", d, m) + w["fc1_b"]
+        hid = 0.5 * hid * (1 + erf(hid / np.sqrt(2)))
+        x = x + w["ls2"] * (hid @ mat("fc2_w", m, d) + w["fc2_b"])
+    return _ln(x, weights["norm_g"], weights["norm_b"], cfg.eps)
+
+
+# options, and what each of them is without: the formulas then give something else
+@pytest.mark.parametrize("kw,others", [
+    (dict(cap=1.0, slopes=[0.5, 0.2]), [dict(cap=None), dict(slopes=None), dict(slopes=[0.5, 0.0]),
+                                        dict(mask="causal")]),
+    (dict(cap=1.0, slopes=[0.5, 0.2], mask="causal"), [dict(cap=None), dict(slopes=[0.0, 0.2]),
+                                                       dict(mask=None)]),
+    (dict(normalized=True), [dict(normalized=False)]),
+    (dict(pairing="half"), [dict(pairing="axis_half")]),
+    (dict(pairing="adjacent", sections=(8, 12, 12)), [dict(pairing="axis_half"),
+                                                      dict(sections=(12, 10, 10))])])
+def test_packed_encoder_options_are_there(kw, others):
+    import torch
+    from beatlm_b200 import model as M
+    cfg = _cfg()
+    w = _weights(cfg, 3)
+    grids = [(1, 9, 11), (2, 4, 6), (1, 1, 1), (1, 13, 10)]
+    rows = sum(t * a * b for t, a, b in grids)
+    x = _patches(cfg, rows, 5)
+    want = _formulas(cfg, w, x[:, :cfg.taps], grids, **kw)
+    far = lambda a: np.linalg.norm(a - want) / np.linalg.norm(want)  # noqa: E731
+    most = cfg.layers * ROUNDINGS * STEP
+    for other in others:
+        assert far(_formulas(cfg, w, x[:, :cfg.taps], grids, **{**kw, **other})) > 3 * most, other
+    enc = M.PackedEncoder(cfg, w, capacity=rows + 3, images=4, dtype="f16", **kw)
+    got = enc.forward(torch.from_numpy(x).half().cuda(),
+                      torch.tensor(grids, dtype=torch.int32).cuda())[:rows].double().cpu().numpy()
+    assert far(got) <= most, far(got)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(cap=1.0, slopes=[0.5, 0.2])])
+def test_packed_encoder_in_bf16(kw):
+    """The default type: bf16 Q and K beside f16 V, steps of 2^-8."""
+    import torch
+    from beatlm_b200 import model as M
+    cfg = _cfg()
+    w = _weights(cfg, 7)
+    grids = [(1, 9, 11), (1, 14, 10), (3, 5, 2)]
+    rows = sum(t * a * b for t, a, b in grids)
+    x = _patches(cfg, rows, 5)
+    want = _formulas(cfg, w, x[:, :cfg.taps], grids, dtype="bf16", **kw)
+    enc = M.PackedEncoder(cfg, w, capacity=rows, images=3, **kw)
+    got = enc.forward(torch.from_numpy(x).bfloat16().cuda(),
+                      torch.tensor(grids, dtype=torch.int32).cuda())[:rows].double().cpu().numpy()
+    rel = np.linalg.norm(got - want) / np.linalg.norm(want)
+    assert rel <= cfg.layers * ROUNDINGS * 2.0 ** -8, rel
