@@ -51,7 +51,7 @@ struct Params {
     long long pos_row;
     int pos_axes;
     int splits;         // CTAs of a cluster that share the keys
-    int chunks;         // query chunks (or tiles) a sequence has at most
+    int chunks;         // query tiles a sequence has at most
     int ragged;         // the sequences' lengths are in device memory
     int mixed;          // a cluster splits the keys of long tiles alone
     Status* status;
@@ -201,11 +201,9 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
     // a packed row are neighbours, so memory pages are read while they are open.
     const unsigned work = blockIdx.x / static_cast<unsigned>(p.splits);
     const int split = static_cast<int>(blockIdx.x - work * p.splits);
-    const int unit = static_cast<int>(work / static_cast<unsigned>(p.kv_heads));
-    const int kvh = static_cast<int>(work - static_cast<unsigned>(unit) * p.kv_heads);
-    const int c0 = unit % p.chunks * kMaxRows;
+    int seq = static_cast<int>(work / static_cast<unsigned>(p.kv_heads));
+    const int kvh = static_cast<int>(work - static_cast<unsigned>(seq) * p.kv_heads);
     // the longest streams first: their CTAs are not the last to start
-    int seq = unit / p.chunks;
     if (p.ragged && p.batch <= 32) {
         const int len = span_of(p, min(lane, p.batch - 1)).len;
         int longer = lane < p.batch ? 0 : p.batch;
@@ -216,8 +214,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
         seq = __ffs(__ballot_sync(kFull, longer == seq && lane < p.batch)) - 1;
     }
     const Span q = span_of(p, seq);
-    const int rows = min((q.len - q.first) * p.group - c0, kMaxRows);
-    if (rows <= 0) return;  // the whole cluster leaves
+    const int rows = (q.len - q.first) * p.group;  // at most kMaxRows
+    if (rows == 0) return;  // the whole cluster leaves
     if (p.splits > 1) {
         if (threadIdx.x == 0) {
             mbar_init(smem_u32(&parts_full), p.splits - 1);
@@ -227,8 +225,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
         cluster_arrive();  // waited for before the parts are sent
     }
 
-    const int most = visible(p, q, q.first + (c0 + rows - 1) / p.group);  // of the last row
-    const int least = visible(p, q, q.first + c0 / p.group);               // of the first
+    const int most = visible(p, q, q.len - 1);  // of the last row
+    const int least = visible(p, q, q.first);   // of the first
     const int tiles = (most + kRowTile - 1) / kRowTile;
     const int first = static_cast<int>(static_cast<unsigned>(tiles) * split / p.splits);
     const int last = static_cast<int>(static_cast<unsigned>(tiles) * (split + 1) / p.splits);
@@ -268,7 +266,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
     uint32_t qa[HD / 16][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        const int c = c0 + min(g + 8 * r, rows - 1);
+        const int c = min(g + 8 * r, rows - 1);
         const int head = kvh * p.group + c % p.group;
         row[r] = q.first + c / p.group;
         seen[r] = visible(p, q, row[r]);
@@ -431,9 +429,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
     }
     __syncthreads();
     auto put = [&](int r, int e, float v) {
-        const int c = c0 + r;
-        const long long at = (q.begin + q.first + c / p.group) * p.out_row +
-                             (kvh * p.group + c % p.group) * HD + e;
+        const long long at = (q.begin + q.first + r / p.group) * p.out_row +
+                             (kvh * p.group + r % p.group) * HD + e;
         if (p.out_dtype == BL_F32) static_cast<float*>(p.out)[at] = v;
         else if (p.out_dtype == BL_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
         else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
@@ -1467,9 +1464,8 @@ Params params_of(const bl_masked_attention_args& a) {
 
 int prepare_rows(const bl_masked_attention_args& a, Launch* out) {
     Params p = params_of(a);
-    const uint64_t combos = 1ull * p.last_rows * p.group;
-    p.chunks = static_cast<int>((combos + kMaxRows - 1) / kMaxRows);
-    const uint64_t units = 1ull * p.chunks * a.batch, ctas = units * p.kv_heads;
+    const uint64_t combos = 1ull * p.last_rows * p.group;  // at most kMaxRows
+    const uint64_t ctas = 1ull * a.batch * p.kv_heads;
     // Splits: as many as run at once (three CTAs an SM), each with 256 keys at
     // least; where that leaves three or fewer and the streams are long, about 768
     // CTAs, so that lengths that differ, and a wave that is not full, even out.
@@ -1482,8 +1478,7 @@ int prepare_rows(const bl_masked_attention_args& a, Launch* out) {
     if (ctas * p.splits > 0x7FFFFFFFull)
         return fail(BL_ERR_UNSUPPORTED, "masked attention: grid too large");
     auto kern = a.qk_dtype == BL_BF16 ? rows_kernel<true> : rows_kernel<false>;
-    const size_t smem = kRowRing + (p.splits > 1 ? p.splits * std::min<uint64_t>(combos, kMaxRows) *
-                                                       kPartFloats * sizeof(float) : 0);
+    const size_t smem = kRowRing + (p.splits > 1 ? p.splits * combos * kPartFloats * sizeof(float) : 0);
     BL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      static_cast<int>(kRowRing + 8 * kMaxRows * kPartFloats *
                                                                      sizeof(float))));
