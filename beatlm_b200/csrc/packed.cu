@@ -87,14 +87,15 @@ __device__ __forceinline__ float centre(float x, float n, float inverse) {
     const float q = x * inverse;
     return fmaf(fmaf(-q, n, x), inverse, q);
 }
-// u / n and its remainder for whole u, n in [0, 2^22): the quotient estimated
-// from the reciprocal is off by one at most, the remainder exact.
+// u / n and its remainder for whole u in [0, 2^22) and n in [1, 2^22]: the whole
+// number nearest to u times the reciprocal. The reciprocal's rounding moves u / n
+// by at most 2^22 2^-24 / n, so that number is within 1/2 + 1/(4 n) of it: the
+// quotient, or one more where the remainder (exact) comes out negative.
 __device__ __forceinline__ float divide(float u, float n, float inverse, float& rest) {
     const float magic = 12582912.0f;  // 1.5 2^23: the sum is a whole number
-    float q = fmaf(u, inverse, magic - 0.5f) - magic;
+    float q = fmaf(u, inverse, magic) - magic;
     rest = fmaf(-q, n, u);
     if (rest < 0.0f) q -= 1.0f, rest += n;
-    if (rest >= n) q += 1.0f, rest -= n;
     return q;
 }
 
