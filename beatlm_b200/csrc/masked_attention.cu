@@ -105,7 +105,9 @@ __device__ __forceinline__ unsigned long long both(float v) { return f2pack(v, v
 // absolute error of a few 2^-23 cap, so a few 2^-21 of the value, for any cap;
 // it goes to +-cap at the ends without a branch. Where the whole tile of a warp
 // is below the limit (`small`) the series alone spares the unit that the
-// exponentials need two of its three functions a score.
+// exponentials need two of its three functions a score: 8 images of up to 1600
+// rows, 16 heads, distances on the grid, take 147 us with scores below a quarter
+// of their cap and 228 to 241 with scores that pass it.
 constexpr float kSmallTanh = 0.25f;
 __device__ __forceinline__ float capped_far(float s, const Capping& k) {
     return fmaf(rcp_approx(1.0f + ex2(s * k.twice)), -2.0f * k.cap2, k.cap2);
@@ -147,8 +149,10 @@ __device__ __forceinline__ float capped(float s, const Capping& k) {
 // running maximum is exact here), which costs 2^-11 of each at most. Warps are
 // merged once at the end; the CTAs of a cluster send their rows' parts into the
 // first one's shared memory and leave, and that adds them in rank order.
-// 16 streams of up to 8192 rows, 16 heads over 8 K/V heads (155 MB): 31.2 us,
-// 76% of a copy's rate (on the FMA units 86.5). Three stages take a fifth
+// 16 streams of up to 8192 rows, 16 heads over 8 K/V heads (160 MB): 31.2 us,
+// 79% of a copy's rate (on the FMA units 86.5), whether the scores reach their
+// cap or not; with positions, which are loaded a key at a time where they are
+// used, 52.6 us for two axes and 57.4 for three. Three stages take a fifth
 // longer (fewer CTAs an SM), 16-key tiles with four 15%.
 constexpr int kRowWarps = 4;
 constexpr int kRowTile = 32;    // keys of a tile
@@ -487,8 +491,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
 //
 // One CTA computes 128 query rows of one head over a range of 64-key tiles on
 // the tensor cores; two CTAs share an SM, with half the TMEM each. The
-// exponentials bound it (one a score at 16 a clock and SM, against a quarter
-// of that time for its products), so the rest is there to keep that unit fed.
+// exponentials bound it (one a score at 16 a clock and SM, against half of that
+// time for its products), so the rest is there to keep that unit fed.
 // Every query row has two softmax threads, one for the even key tiles and one
 // for the odd, so four softmax warps a scheduler cover one another's waits;
 // S has three TMEM buffers, so the scores of the next tile are there before a
@@ -506,11 +510,14 @@ __global__ void __launch_bounds__(32 * kRowWarps) rows_kernel(const __grid_const
 // A thread reads its 64 scores from TMEM twice, 32 at a time, for the maximum
 // and for the exponentials (a 32-column load takes 17 clocks of a warp
 // scheduler's TMEM port, 32 exponentials 256), which leaves it within the 96
-// registers that ten warps and two CTAs allow.
-// One sequence of 10960 rows, 16 heads: 632 us, 778 TFLOP/s; the exponentials'
-// unit is busy for 78% of a step (776 clocks of an SM for 128 x 64 scores, 512
-// at its rate; the rest is the softmax threads' way from S to the running
-// maximum, which the four of a scheduler cover in part). Making an eighth to a
+// registers that ten warps and two CTAs allow. P is rounded to f16, the type of V
+// (an instruction takes one type), by 2^-11 of a probability at most or by 2^-25
+// of the reference below f16's normal range; its sum is of the f32 values.
+// One sequence of 10960 rows, 16 heads: 632 us, 778 TFLOP/s in short runs at
+// 1965 MHz (692 in long ones, at the power cap); the exponentials' unit is busy
+// for 66% of a step (776 clocks of an SM for 128 x 64 scores, 512 at its rate;
+// the rest is the softmax threads' way from S to the running maximum, which the
+// four of a scheduler cover in part). Making an eighth to a
 // third of the exponentials by a polynomial on the FMA units lengthens that way
 // and takes 645 to 670 us. A CTA's start and end cost 9000 clocks beside its steps.
 // Tiles start at their sequence's first row, so a key tile holds keys of one
