@@ -552,8 +552,9 @@ struct LeanOperands {
     uint8_t key[2][BN * 32];     // B: row k holds k (or -k) three times, twice
 };
 
+static_assert((kQBytes + 2 * STAGES * kKvBytes) % 1024 == 0, "the tail starts on a swizzle atom");
 struct TileTail {
-    alignas(1024) union {
+    union {  // first, so that matrix operands and 16-byte loads are aligned
         LeanOperands lean;
         float kpos[8][3][BN];  // each softmax warp's copy of a key tile's positions, negated
     };
