@@ -838,7 +838,8 @@ class PackedEncoder:
     in place, attention by image, out-projection, LayerNorm and the MLP's two
     GEMMs (the block of ``block_specs`` with two kernels more), and the final
     LayerNorm. Everything is prebuilt once: sizes are device data, so one
-    program (or its graph) runs every batch that fits."""
+    program (or its graph) runs every batch that fits. After a pass ``offsets``
+    and ``image_of`` say whose the rows of ``out`` are."""
 
     def __init__(self, cfg: ViTConfig, weights: dict, capacity: int, images: int,
                  dtype: str = "bf16", device="cuda", sections=None, theta: float = 100.0,
